@@ -14,11 +14,16 @@ new tokens and earlier tokens each sequence has; `own` selects the framework's k
 `run` is the plain form in elementary torch operations.
 """
 import math
+import os
 import random
+import sys
 
 import torch
 
 own = False
+
+# the package's folder is not importable by name; the working folder is the repository's root
+PACKAGE = os.path.join(os.getcwd(), "qwen-mtp-mac_b200")
 
 BF16 = torch.bfloat16
 
@@ -176,6 +181,8 @@ def prepare(case, seed):
         st["q"] = normal(tokens, nq, dh, scale=1.3)
         st["gate"] = normal(tokens, nq, 2, dh)[:, :, 1] if case["gated"] else None
     if own:
+        if PACKAGE not in sys.path:
+            sys.path.insert(0, PACKAGE)
         from qmtp import paged
 
         st["cache"] = paged.PagedCache(st["k"], st["v"])
