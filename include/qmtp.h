@@ -425,6 +425,75 @@ int qmtp_moe_dispatch(const void* idx, int T, int S, const void* x, int H, int n
                       int cap, void* send_x, void* send_e, void* sh_x, void* sh_e, void* pos, void* counts,
                       void* stream);
 
+/* --------------------------------------------------------------------------------------------
+ * Attention over a key/value cache kept in pages (no counterpart in the reference, which serves one
+ * conversation from contiguous caches, mtp.py:143-153): several sequences share one pool of pages.
+ *   k, v      bf16 [pages, n_kv, page, Dh], contiguous, 16-byte aligned; Dh 64, 128 or 256; page a
+ *             power of two, 16 .. 256; pages * n_kv * page < 2^31
+ *   table     int32 [B, ld_table]: position p of sequence b lives in page table[b][p / page], row p % page
+ *             (the first table_w entries of a row are used; only entries of pages that are read or
+ *             written are looked at, so pages that fell out of a sliding window may be given away)
+ *   lens      int32 [B]: tokens of each sequence in the cache, this call's new tokens included
+ *   B         sequences, 1 .. 4096
+ * table and lens are read on the device when the call runs, so a captured graph follows them.  The new
+ * tokens of sequence b are its last n_b positions lens[b] - n_b .. lens[b] - 1.  A sequence with
+ * lens[b] == 0 is empty.  Bad device-side values never read or write outside the arrays: they set bit 1
+ * of the device error word, and a sequence whose length is negative or above table_w * page counts as
+ * empty, a row of a page outside [0, pages) is read as zeros and not written. */
+typedef struct qmtp_paged_cache {
+  void* k;
+  void* v;
+  const int* table;
+  const int* lens;
+  long long pages;
+  long long ld_table;
+  int n_kv, page, Dh, table_w, B;
+} qmtp_paged_cache;
+
+/* Per-head RMS norm of queries and keys, rotate-half position rotation and the cache write in one
+ * pass over the projection output (qmtp_attn_prep's work for a ragged batch, any head layout):
+ *   qkv    bf16 [T, ld]: n_q heads of q (gated: (q, gate) pairs, as qmtp_attn_prep), n_kv of k, n_kv of v
+ *   cu     int32 [B + 1] or NULL: rows cu[b] .. cu[b+1] are the new tokens of sequence b, in order; rows
+ *          outside [cu[0], cu[B]) belong to no sequence.  NULL: T = B * n, n rows for every sequence
+ *   q_w, k_w  bf16 [Dh] norm weights, NULL: no norm;  cos_t, sin_t fp32 [max_pos, rotary / 2], NULL (both):
+ *          no rotation; rotary a multiple of 16, 16 .. Dh
+ *   q_out  bf16 [T, n_q, Dh].  All arithmetic in fp32, one rounding per output; v is copied.
+ * A row of no sequence, or at a negative position (a sequence shorter than its row count), is skipped:
+ * q_out keeps what it held there.  A position at or above max_pos is skipped too and sets the error word.
+ * ld % 8 == 0; qkv, q_w, k_w, cos_t, sin_t, q_out 16-byte aligned. */
+int qmtp_paged_append(const void* qkv, long long ld, int T, const int* cu, int n_q, int gated, const void* q_w,
+                      const void* k_w, float eps, const float* cos_t, const float* sin_t, int rotary, int max_pos,
+                      void* q_out, const qmtp_paged_cache* cache, void* stream);
+
+/* What both attention calls share: softmax(scale * q . k) over the keys a query sees, times v, per head
+ * (query head h reads key head h / (n_q / n_kv)), and with a gate times sigmoid(gate).  The query at
+ * position p sees key j <= p when window == 0, or p - j < window, or j < sinks.  A query that sees no
+ * key (an empty sequence, a negative position) gives zeros.  Keys and values a query does not see never
+ * reach its output, whatever they hold (infinities and NaN included).
+ *   q     bf16 [T, n_q, Dh], rows q_ld elements apart (0: n_q * Dh)
+ *   gate  bf16 or NULL: head h of row t at gate + t * gate_ld + h * gate_hs (elements), e.g. the gates
+ *         that qmtp_paged_append leaves in qkv
+ *   out   bf16 [T, n_q * Dh]
+ * scale > 0 and finite; window, sinks >= 0; q, gate, out 16-byte aligned, strides multiples of 8. */
+typedef struct qmtp_paged_args {
+  const void* q;
+  const void* gate;
+  void* out;
+  long long q_ld, gate_ld, gate_hs;
+  int T, n_q;
+  float scale;
+  int window, sinks;
+} qmtp_paged_args;
+
+/* Attention of the newest tokens: T = B * S rows, row b * S + s at position lens[b] - S + s; S <= 8,
+ * n_q / n_kv <= 64.  A sequence's keys are cut into slabs at fixed positions, the slabs are computed all
+ * over the GPU and joined in order, so a token's result has the same bits whatever B, S, the page size
+ * and the other sequences are.  workspace: qmtp_paged_attention_workspace bytes, 16-byte aligned (two
+ * calls that may run at the same time need their own). */
+size_t qmtp_paged_attention_workspace(const qmtp_paged_args* args, const qmtp_paged_cache* cache);
+int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_paged_cache* cache, void* workspace,
+                         size_t ws_bytes, void* stream);
+
 /* Control block of the device-side speculative loop (int32 [QMTP_CTRL_SIZE]). */
 #define QMTP_CTRL_SLOT 0      /* GatedDeltaNet state ring slot before the next verify */
 #define QMTP_CTRL_CONV_ROW 1  /* row of the conv state inside the [2 * win_rows, C] window buffer */

@@ -1,0 +1,116 @@
+// Shared pieces of the paged-cache kernels (paged.cu, paged_prompt.cu): the device view of a cache,
+// which keys a query sees, and the strict evaluation of one attention row.
+#pragma once
+#include <atomic>
+
+#include "common.cuh"
+
+namespace qmtp {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxSeqs = 4096;
+
+// Device view of qmtp_paged_cache.  page = 1 << page_log.
+struct PagedView {
+  uint16_t* k;
+  uint16_t* v;
+  const int* table;
+  const int* lens;
+  long long pages, ld_table;
+  int nkv, page_log, table_w, B;
+};
+
+// Which keys a query at position p sees (qmtp_paged_args): j <= p and (no window, or p - j < window, or j < sinks).
+struct Visible {
+  int window, sinks;
+  __device__ __forceinline__ bool operator()(int p, int j) const {
+    return j <= p && (window == 0 || p - j < window || j < sinks);
+  }
+  // first key of the window of the query at position p (0 without a window)
+  __device__ __forceinline__ int first(int p) const { return window == 0 || p - window + 1 < 0 ? 0 : p - window + 1; }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Length of sequence b: a value the table cannot hold counts as empty (and is reported).
+__device__ __forceinline__ int seq_len(const PagedView& c, int b, unsigned* err) {
+  const int n = c.lens[b];
+  if (n < 0 || n > ((long long)c.table_w << c.page_log)) {
+    if (err) atomicOr(err, DEVERR_BADARG);
+    return 0;
+  }
+  return n;
+}
+
+// Row index (of Dh elements) of position j of sequence b, head kh, in k and v; -1 for a bad page.
+__device__ __forceinline__ long long cache_row(const PagedView& c, int b, int kh, int j, unsigned* err) {
+  const long long pg = c.table[(long long)b * c.ld_table + (j >> c.page_log)];
+  if (pg < 0 || pg >= c.pages) {
+    atomicOr(err, DEVERR_BADARG);
+    return -1;
+  }
+  return ((pg * c.nkv + kh) << c.page_log) + (j & ((1 << c.page_log) - 1));
+}
+
+// One query row over the keys [j0, j1) of its sequence that it sees, by one warp: lane l owns dims
+// [l * Dh / 32, (l + 1) * Dh / 32).  One pass with the running maximum m (base 2) and sum l of the softmax;
+// o is the numerator.  Only rows that are seen are read, so nothing behind the mask can reach o.
+template <int Dh>
+__device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t* __restrict__ qrow, int b, int kh,
+                                               int p, int j0, int j1, Visible vis, float scale2, unsigned* err,
+                                               float& m, float& l, float (&o)[Dh / 32]) {
+  constexpr int N = Dh / 32;
+  const int lane = threadIdx.x & 31;
+  float q[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    q[e] = bf2f(qrow[lane * N + e]);
+    o[e] = 0.0f;
+  }
+  m = __int_as_float(0xFF800000);
+  l = 0.0f;
+  for (int j = j0; j < j1; ++j) {
+    if (!vis(p, j)) continue;
+    const long long r = cache_row(c, b, kh, j, err);
+    float s = 0.0f;
+    if (r >= 0)
+#pragma unroll
+      for (int e = 0; e < N; ++e) s = __fmaf_rn(q[e], bf2f(c.k[r * Dh + lane * N + e]), s);
+    s = __fmul_rn(warp_sum(s), scale2);
+    const float mn = fmaxf(m, s);
+    const float safe = mn == __int_as_float(0xFF800000) ? 0.0f : mn;
+    const float a = exp2f(__fsub_rn(m, safe)), w = exp2f(__fsub_rn(s, safe));
+    l = __fmaf_rn(l, a, w);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = r >= 0 ? bf2f(c.v[r * Dh + lane * N + e]) : 0.0f;
+      o[e] = __fmaf_rn(w, x, __fmul_rn(o[e], a));
+    }
+    m = mn;
+  }
+}
+
+// Runs a set-up call (a kernel's attributes) once for every device the process uses; false if it failed,
+// and a failure is tried again by the next call.
+struct DeviceOnce {
+  std::atomic<bool> done[64] = {};
+  template <typename F>
+  bool operator()(F f) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (done[dev].load(std::memory_order_acquire)) return true;
+    if (f() != cudaSuccess) return false;
+    done[dev].store(true, std::memory_order_release);
+    return true;
+  }
+};
+
+// Host checks shared by the entry points; fills the device view.
+int paged_view(const qmtp_paged_cache* cache, PagedView* out);
+int paged_check_args(const qmtp_paged_args* a, const qmtp_paged_cache* c);
+
+}  // namespace qmtp

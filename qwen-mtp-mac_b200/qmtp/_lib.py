@@ -116,6 +116,25 @@ class SamplingArgs(ctypes.Structure):
 SIGNATURES["qmtp_sample"] = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                              ctypes.c_int, ctypes.c_int, ctypes.POINTER(SamplingArgs), ctypes.c_int,
                              ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """Mirror of qmtp_paged_cache (include/qmtp.h)."""
+    _fields_ = [("k", _P), ("v", _P), ("table", _P), ("lens", _P), ("pages", ctypes.c_longlong),
+                ("ld_table", ctypes.c_longlong), ("n_kv", _I), ("page", _I), ("Dh", _I), ("table_w", _I), ("B", _I)]
+
+
+class PagedArgs(ctypes.Structure):
+    """Mirror of qmtp_paged_args (include/qmtp.h)."""
+    _fields_ = [("q", _P), ("gate", _P), ("out", _P), ("q_ld", ctypes.c_longlong), ("gate_ld", ctypes.c_longlong),
+                ("gate_hs", ctypes.c_longlong), ("T", _I), ("n_q", _I), ("scale", _F), ("window", _I), ("sinks", _I)]
+
+
+SIGNATURES.update({
+    "qmtp_paged_append": [_P, ctypes.c_longlong, _I, _P, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P,
+                          ctypes.POINTER(PagedCacheArgs), _P],
+    "qmtp_paged_attention": [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedCacheArgs), _P, ctypes.c_size_t, _P],
+})
 CTRL_SIZE = 32
 # size queries return size_t
 SIZE_QUERIES: dict[str, list] = {
@@ -125,6 +144,7 @@ SIZE_QUERIES: dict[str, list] = {
     "qmtp_topk_workspace": [_I, _I, _I],
     "qmtp_argmax_workspace": [_I, _I],
     "qmtp_moe_workspace": [_I, _I, _I, _I, _I],
+    "qmtp_paged_attention_workspace": [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedCacheArgs)],
 }
 
 _lib = None
