@@ -494,6 +494,15 @@ size_t qmtp_paged_attention_workspace(const qmtp_paged_args* args, const qmtp_pa
 int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_paged_cache* cache, void* workspace,
                          size_t ws_bytes, void* stream);
 
+/* Attention of a ragged batch of prompt chunks: rows cu[b] .. cu[b+1] of q (int32 [B + 1], in [0, T]) are
+ * the last tokens of sequence b, whose keys and values are already in the cache (qmtp_paged_append).
+ * Runs on the tensor cores (tcgen05).  Rows of out outside every sequence are left as they were.
+ * n_q / n_kv <= 64.  workspace: qmtp_paged_prompt_workspace bytes, 16-byte aligned (two calls that may run
+ * at the same time need their own): with few rows the keys are split over CTAs and joined. */
+size_t qmtp_paged_prompt_workspace(const qmtp_paged_args* args, const qmtp_paged_cache* cache);
+int qmtp_paged_prompt(const qmtp_paged_args* args, const int* cu, const qmtp_paged_cache* cache, void* workspace,
+                      size_t ws_bytes, void* stream);
+
 /* Control block of the device-side speculative loop (int32 [QMTP_CTRL_SIZE]). */
 #define QMTP_CTRL_SLOT 0      /* GatedDeltaNet state ring slot before the next verify */
 #define QMTP_CTRL_CONV_ROW 1  /* row of the conv state inside the [2 * win_rows, C] window buffer */

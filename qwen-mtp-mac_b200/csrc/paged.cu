@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(128, Dh == 256 ? 2 : 4) paged_decode_kernel(Pa
       // Settle it by the definition, a warp per row, reading visible keys only.
       for (int n = warp; n < 8 * NT && row0 + n < R; n += 4) {
         const int r = row0 + n, s = r / a.G, h = kh * a.G + r - s * a.G;
-        float mm, ll, oo[Dh / 32];
+        float mm = -INFINITY, ll = 0.0f, oo[Dh / 32] = {};
         attend_row_strict<Dh>(c, a.q + (long long)(b * a.S + s) * a.q_ld + (long long)h * Dh, b, kh, pos0 + s, k_begin,
                               k_end, a.vis, a.scale2, a.err, mm, ll, oo);
         for (int e = 0; e < Dh / 32; ++e) store(r, lane * (Dh / 32) + e, oo[e], ll);

@@ -2,6 +2,7 @@
 // which keys a query sees, and the strict evaluation of one attention row.
 #pragma once
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -27,7 +28,7 @@ struct Visible {
     return j <= p && (window == 0 || p - j < window || j < sinks);
   }
   // first key of the window of the query at position p (0 without a window)
-  __device__ __forceinline__ int first(int p) const { return window == 0 || p - window + 1 < 0 ? 0 : p - window + 1; }
+  __device__ __forceinline__ int first(int p) const { return window == 0 || window > p ? 0 : p - window + 1; }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -57,8 +58,9 @@ __device__ __forceinline__ long long cache_row(const PagedView& c, int b, int kh
 }
 
 // One query row over the keys [j0, j1) of its sequence that it sees, by one warp: lane l owns dims
-// [l * Dh / 32, (l + 1) * Dh / 32).  One pass with the running maximum m (base 2) and sum l of the softmax;
-// o is the numerator.  Only rows that are seen are read, so nothing behind the mask can reach o.
+// [l * Dh / 32, (l + 1) * Dh / 32).  One pass with the running maximum m (base 2), sum l and numerator o of
+// the softmax, which the caller starts at (-inf, 0, 0).  Only rows that are seen are read, so nothing
+// behind the mask can reach o.
 template <int Dh>
 __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t* __restrict__ qrow, int b, int kh,
                                                int p, int j0, int j1, Visible vis, float scale2, unsigned* err,
@@ -67,13 +69,8 @@ __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t
   const int lane = threadIdx.x & 31;
   float q[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    q[e] = bf2f(qrow[lane * N + e]);
-    o[e] = 0.0f;
-  }
-  m = __int_as_float(0xFF800000);
-  l = 0.0f;
-  for (int j = j0; j < j1; ++j) {
+  for (int e = 0; e < N; ++e) q[e] = bf2f(qrow[lane * N + e]);
+  for (int j = j0; j < j1 && j <= p; ++j) {
     if (!vis(p, j)) continue;
     const long long r = cache_row(c, b, kh, j, err);
     float s = 0.0f;
@@ -82,7 +79,7 @@ __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t
       for (int e = 0; e < N; ++e) s = __fmaf_rn(q[e], bf2f(c.k[r * Dh + lane * N + e]), s);
     s = __fmul_rn(warp_sum(s), scale2);
     const float mn = fmaxf(m, s);
-    const float safe = mn == __int_as_float(0xFF800000) ? 0.0f : mn;
+    const float safe = mn == -INFINITY ? 0.0f : mn;
     const float a = exp2f(__fsub_rn(m, safe)), w = exp2f(__fsub_rn(s, safe));
     l = __fmaf_rn(l, a, w);
 #pragma unroll

@@ -134,6 +134,7 @@ SIGNATURES.update({
     "qmtp_paged_append": [_P, ctypes.c_longlong, _I, _P, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P,
                           ctypes.POINTER(PagedCacheArgs), _P],
     "qmtp_paged_attention": [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedCacheArgs), _P, ctypes.c_size_t, _P],
+    "qmtp_paged_prompt": [ctypes.POINTER(PagedArgs), _P, ctypes.POINTER(PagedCacheArgs), _P, ctypes.c_size_t, _P],
 })
 CTRL_SIZE = 32
 # size queries return size_t
@@ -145,6 +146,7 @@ SIZE_QUERIES: dict[str, list] = {
     "qmtp_argmax_workspace": [_I, _I],
     "qmtp_moe_workspace": [_I, _I, _I, _I, _I],
     "qmtp_paged_attention_workspace": [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedCacheArgs)],
+    "qmtp_paged_prompt_workspace": [ctypes.POINTER(PagedArgs), ctypes.POINTER(PagedCacheArgs)],
 }
 
 _lib = None

@@ -179,3 +179,22 @@ def attention(q, cache: PagedCache, table, lens, *, gate=None, scale: float | No
         _lib.check(L.qmtp_paged_attention(ctypes.byref(a), ctypes.byref(c), _lib.ptr(ws), n, _lib.stream()),
                    "paged attention")
     return out
+
+
+def prompt_attention(q, cache: PagedCache, table, lens, cu, *, gate=None, scale: float | None = None, window: int = 0,
+                     sinks: int = 0, out=None):
+    """Attention of a ragged batch of prompt chunks: rows cu[b] .. cu[b+1] of q bf16 [T, heads, head_dim] are the
+    last tokens of sequence b -> bf16 [T, heads * head_dim].  Masks, scale and gate as in ``attention``; rows of
+    no sequence are left as they were.  Any number of new tokens per sequence; ``attention`` is the one for a few."""
+    a, out = _attention_args(q, cache, gate, scale, window, sinks, out)
+    _check_cu(cu, table.shape[0], cache.k.device)
+    if q.shape[0] == 0:
+        return out
+    c = cache._args(table, lens)
+    L = _lib.lib()
+    with torch.cuda.device(cache.k.device):
+        n = L.qmtp_paged_prompt_workspace(ctypes.byref(a), ctypes.byref(c))
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _lib.check(L.qmtp_paged_prompt(ctypes.byref(a), cu.data_ptr(), ctypes.byref(c), _lib.ptr(ws), n, _lib.stream()),
+                   "paged prompt attention")
+    return out

@@ -45,6 +45,7 @@ def test_cache_refusals(change, code):
 
     L, c = _lib.lib(), cache(**change)
     assert L.qmtp_paged_attention(ctypes.byref(attn()), ctypes.byref(c), PTR, 1 << 30, None) == code
+    assert L.qmtp_paged_prompt(ctypes.byref(attn()), PTR, ctypes.byref(c), PTR, 1 << 30, None) == code
     assert L.qmtp_paged_append(PTR, 2048, 4, None, 4, 0, None, None, 1e-6, None, None, 0, 0, PTR, ctypes.byref(c), None) == code
 
 
@@ -53,6 +54,15 @@ def test_attention_refusals(change, code):
     from qmtp import _lib
 
     assert _lib.lib().qmtp_paged_attention(ctypes.byref(attn(**change)), ctypes.byref(cache()), PTR, 1 << 30, None) == code
+
+
+@pytest.mark.parametrize("change,code", BAD_ATTN)
+def test_prompt_refusals(change, code):
+    from qmtp import _lib
+
+    L = _lib.lib()
+    assert L.qmtp_paged_prompt(ctypes.byref(attn(**change)), PTR, ctypes.byref(cache()), PTR, 1 << 30, None) == code
+    assert L.qmtp_paged_prompt(ctypes.byref(attn()), None, ctypes.byref(cache()), PTR, 1 << 30, None) == ARG
 
 
 def test_attention_workspace():
