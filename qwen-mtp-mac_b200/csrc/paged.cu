@@ -135,10 +135,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
 // A unit of work is (sequence, slab of keys, key head, tile of query rows); rows are the S tokens x G query
 // heads of the key head.  Scores and the weighted sum run on the tensor cores with the keys (dims) on the
 // M side, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so a group of 4 or 8 rows fills the 8-wide N side.
-// The keys' bytes bound it (4 flops a byte and row group), so mma.sync, fed from a ring that cp.async
-// keeps full, is enough: its pipe is a small part of the time the bytes take.
+// The keys' bytes bound it (4 flops a byte and row group), so mma.sync is enough: its pipe is a small part of the
+// time the bytes take.  A CTA takes units u, u + grid, ...; its producer warp walks their tiles ahead of the four
+// consumer warps and keeps the ring full across units, so neither a unit's first load nor its table
+// lookups are waited for.
 constexpr int kTile = 64;      // keys per step: 16 a warp for the scores
-constexpr int kRing = 3;       // ring entries: a tile of K or of V each
 constexpr int kFineSlab = 128; // slab sizes: see slab_of
 constexpr int kFineKeys = 4096;
 constexpr int kSlab = 512;
@@ -169,15 +170,14 @@ struct DecodeArgs {
 
 // Slabs of one sequence that some query row of it sees: [0, first) and [from, from + count - first).
 struct SlabList {
-  int len, lo, first, from, count;
+  int lo, first, from, count;
 };
-__device__ __forceinline__ SlabList slab_list(const PagedView& c, const DecodeArgs& a, int b, unsigned* err) {
+__device__ __forceinline__ SlabList slab_list(const DecodeArgs& a, int len) {
   SlabList s;
-  s.len = seq_len(c, b, err);
-  s.lo = a.vis.first(max(0, s.len - a.S));  // the first key of the oldest row's window
+  s.lo = a.vis.first(max(0, len - a.S));  // the first key of the oldest row's window
   s.from = slab_of(s.lo, a.fine);
   s.first = a.vis.sinks > 0 && s.lo > 0 ? min(slab_of(min(a.vis.sinks, s.lo) - 1, a.fine) + 1, s.from) : 0;
-  s.count = s.len > 0 ? s.first + slab_of(s.len - 1, a.fine) + 1 - s.from : 1;  // an empty sequence: one empty slab
+  s.count = len > 0 ? s.first + slab_of(len - 1, a.fine) + 1 - s.from : 1;  // an empty sequence: one empty slab
   return s;
 }
 
@@ -199,194 +199,278 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 16-byte asynchronous copy; zeros when !live
-__device__ __forceinline__ void cp_async16_z(uint32_t dst, const void* src, bool live) {
-  const int n = live ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// Barrier of the four consumer warps.
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <int Dh, int NT>
-struct DecodeSmem {
-  uint16_t kv[kRing][kTile * Dh];  // 16-byte chunk x of row r sits at chunk x ^ (r & 7)
-  uint16_t p[8 * NT][kTile + 8];   // weights, [row][key]
-  float mx[4][8 * NT];
-  float sum[4][8 * NT];
-  int scan[4];
-  int bad;
+template <int Dh>
+struct DecodeCfg {
+  static constexpr int ring = Dh == 256 ? 3 : Dh == 128 ? 4 : 6;  // entries: a tile of K or of V each
+  static constexpr int per_sm = Dh == 256 ? 2 : Dh == 128 ? 3 : 4;
 };
 
 template <int Dh, int NT>
-__global__ void __launch_bounds__(128, Dh == 256 ? 2 : 4) paged_decode_kernel(PagedView c, DecodeArgs a) {
+struct DecodeSmem {
+  uint16_t kv[DecodeCfg<Dh>::ring][kTile * Dh];  // 64-dim column blocks of 128-byte swizzled rows
+  static constexpr int QS = NT == 2 ? 1 : 2;  // per_sm CTAs have to fit on an SM
+  uint16_t q[QS][8 * NT][Dh + 8];
+  uint16_t p[8 * NT][kTile + 8];  // weights, [row][key]
+  float mx[4][8 * NT];
+  float sum[2][4][8 * NT];
+  uint64_t full[DecodeCfg<Dh>::ring], empty[DecodeCfg<Dh>::ring], q_full[2], q_empty[2];
+  int bad[2];
+  int scan[8];
+  int dead;
+};
+
+struct DecodeUnit {
+  int b, kh, row0, len, lo, k_begin, k_end, part;
+  bool whole;
+};
+
+template <int Dh, int NT>
+__global__ void __launch_bounds__(160, DecodeCfg<Dh>::per_sm)
+paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, PagedView c,
+                    DecodeArgs a) {
   pdl_trigger();
-  pdl_wait();
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  DecodeSmem<Dh, NT>& sm = *reinterpret_cast<DecodeSmem<Dh, NT>*>(smem_raw);
-  int* s_pre = reinterpret_cast<int*>(smem_raw + sizeof(DecodeSmem<Dh, NT>));  // [B + 1] slabs before sequence b
-  constexpr int CPR = Dh / 8;        // 16-byte chunks per row
-  constexpr int RPI = 32 / CPR;      // rows a warp copies per instruction
-  constexpr int MT = Dh / 64;        // 16-dim tiles of a warp in the weighted sum
+  extern __shared__ uint8_t smem_raw[];
+  using Smem = DecodeSmem<Dh, NT>;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  int* s_pre = reinterpret_cast<int*>(&sm + 1);  // [B + 1] slabs before sequence b
+  int* s_len = s_pre + c.B + 1;                  // [B]
+  constexpr int RING = DecodeCfg<Dh>::ring, CB = Dh / 64, QS = Smem::QS;
+  constexpr int MT = Dh / 64;  // 16-dim tiles of a warp in the weighted sum
   constexpr float kNone = -INFINITY;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = lane & 3, oct = lane >> 2;
-  // slabs before every sequence
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 128) {
+    for (int i = 0; i < RING; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sm.q_full[i], 1); mbar_init(&sm.q_empty[i], 4); sm.bad[i] = 0; }
+    sm.dead = 0;
+    fence_mbar_init();
+  }
+  pdl_wait();
   int total = 0;
-  for (int b0 = 0; b0 < c.B; b0 += 128) {
+  for (int b0 = 0; b0 < c.B; b0 += 160) {
     const int b = b0 + tid;
-    const int n = b < c.B ? slab_list(c, a, b, blockIdx.x == 0 ? a.err : nullptr).count : 0;
+    int n = 0, len = 0;
+    if (b < c.B) {
+      len = seq_len(c, b, blockIdx.x == 0 ? a.err : nullptr);
+      n = slab_list(a, len).count;
+    }
     int chunk;
     const int before = block_excl_scan(n, sm.scan, chunk);
-    if (b < c.B) s_pre[b] = total + before;
+    if (b < c.B) { s_pre[b] = total + before; s_len[b] = len; }
     total += chunk;
   }
   if (tid == 0) s_pre[c.B] = total;
   __syncthreads();
-  const int R = a.S * a.G, per = c.nkv * a.row_tiles;
-  const long long units = (long long)total * per;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int slab_g = int(u / per), rest = int(u - (long long)slab_g * per);
-    const int kh = rest / a.row_tiles, row0 = (rest - kh * a.row_tiles) * 8 * NT;
+  const int R = a.S * a.G, per = c.nkv * a.row_tiles, units = total * per;
+  auto unit_at = [&](int u) {
+    DecodeUnit x;
+    const int slab_g = u / per, rest = u - slab_g * per;
+    x.kh = rest / a.row_tiles;
+    x.row0 = (rest - x.kh * a.row_tiles) * 8 * NT;
     int b = 0;  // the last sequence that begins at or before this slab
     for (int step = 1 << (31 - __clz(c.B)); step > 0; step >>= 1)
       if (b + step < c.B && s_pre[b + step] <= slab_g) b += step;
-    const SlabList sl = slab_list(c, a, b, nullptr);
-    const int i_slab = slab_g - s_pre[b];
-    const int slab = i_slab < sl.first ? i_slab : sl.from + i_slab - sl.first;
-    const int k_begin = slab_begin(slab, a.fine), k_end = min(slab_begin(slab + 1, a.fine), sl.len);
-    const int pos0 = sl.len - a.S;
-    // tiles of the slab that hold a needed key
-    auto next_tile = [&](int j) {
-      while (j < k_end && a.vis.window != 0 && j + kTile <= sl.lo && j >= a.vis.sinks) j += kTile;
-      return j;
+    x.b = b;
+    x.len = s_len[b];
+    const SlabList sl = slab_list(a, x.len);
+    x.lo = sl.lo;
+    x.part = slab_g - s_pre[b];
+    const int slab = x.part < sl.first ? x.part : sl.from + x.part - sl.first;
+    x.k_begin = slab_begin(slab, a.fine);
+    x.k_end = min(slab_begin(slab + 1, a.fine), x.len);
+    x.whole = sl.count == 1;  // the only slab: its result is final
+    return x;
+  };
+  // the next tile of the unit, from key j on, that holds a needed key
+  auto next_tile = [&](const DecodeUnit& x, int j) {
+    while (j < x.k_end && a.vis.window != 0 && j + kTile <= x.lo && j >= a.vis.sinks) j += kTile;
+    return j;
+  };
+
+  if (warp == 4) {
+    // -------------------------------------------------------------------- producer
+    const int box = min(1 << c.page_log, kTile), parts = kTile / box;
+    const long long none = (c.pages * c.nkv) << c.page_log;  // past the end: reads as zeros
+    // cache row of part `lane` of the tile at key j; a page that no row needs is not looked at
+    auto part_row = [&](const DecodeUnit& x, int j) -> int {
+      const int key = j + lane * box;
+      if (lane >= parts || key >= x.k_end || (a.vis.window != 0 && key + box <= x.lo && key >= a.vis.sinks))
+        return int(none);
+      const long long r = cache_row(c, x.b, x.kh, key, a.err);
+      return int(r < 0 ? none : r);
     };
-    // rows of this lane: n = 8 t + 2 quad + e (softmax, output), n = 8 t + oct (query fragment)
-    uint32_t qf[NT][Dh / 16][2];
-    int prow[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = row0 + 8 * t + 2 * quad + e;
-        prow[t][e] = r < R ? pos0 + r / a.G : -1;
-      }
-      const int r = row0 + 8 * t + oct;
-      const int s = r / a.G;
-      const uint16_t* qp = a.q + (long long)(b * a.S + s) * a.q_ld + (long long)(kh * a.G + r - s * a.G) * Dh + 2 * quad;
-#pragma unroll
-      for (int k = 0; k < Dh / 16; ++k) {
-        qf[t][k][0] = r < R ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
-        qf[t][k][1] = r < R ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
-      }
+    const int part = lane / CB, cb = lane - part * CB;
+    int e = 0, uq = 0;
+    auto load = [&](const CUtensorMap* map, int row) {
+      const int st = e % RING;
+      bar_wait(&sm.dead, &sm.empty[st], ((e / RING) & 1) ^ 1, a.err);
+      if (*reinterpret_cast<volatile int*>(&sm.dead)) return;
+      if (lane == 0) mbar_expect_tx(&sm.full[st], kTile * Dh * 2);
+      __syncwarp();
+      const int r = __shfl_sync(0xFFFFFFFFu, row, min(part, parts - 1));
+      if (part < parts)
+        tma_load_2d(reinterpret_cast<uint8_t*>(sm.kv[st]) + cb * kTile * 128 + part * box * 128, map, cb * 64, r,
+                    &sm.full[st], policy_evict_first());
+      ++e;
+    };
+    DecodeUnit x;
+    int j = 0, row = 0, u = blockIdx.x;
+    if (u < units) {
+      x = unit_at(u);
+      j = next_tile(x, x.k_begin);
+      if (j < x.k_end) row = part_row(x, j);
     }
-    // row of the caches that this lane's key (16 warp + lane % 16) of the tile at j lies in, -1: none needed
-    auto key_row = [&](int j) -> long long {
-      const int key = j + 16 * warp + (lane & 15);
-      if (key >= k_end || (a.vis.window != 0 && key < sl.lo && key >= a.vis.sinks)) return -1;
-      return cache_row(c, b, kh, key, a.err);
-    };
-    auto load = [&](int slot, const uint16_t* base, long long r_lane) {
-      const uint32_t dst = smem_u32(sm.kv[slot]);
-#pragma unroll
-      for (int i = 0; i < 16 / RPI; ++i) {
-        const int rr = i * RPI + lane / CPR;  // row of the warp's 16
-        const long long r = __shfl_sync(0xFFFFFFFFu, r_lane, rr);
-        const int row = 16 * warp + rr, ch = lane % CPR;
-        cp_async16_z(dst + row * Dh * 2 + ((ch ^ (row & 7)) << 4), base + (r < 0 ? 0 : r) * Dh + ch * 8, r >= 0);
+    bool head = true;
+    while (u < units && !*reinterpret_cast<volatile int*>(&sm.dead)) {
+      // the tile after this one, its table entries on their way while this one's copies are issued
+      DecodeUnit xn = x;
+      int un = u, jn = j < x.k_end ? next_tile(x, j + kTile) : x.k_end;
+      if (jn >= x.k_end) {
+        un = u + gridDim.x;
+        if (un < units) {
+          xn = unit_at(un);
+          jn = next_tile(xn, xn.k_begin);
+        }
       }
-    };
-    // ring order K0 V0 K1 V1 ...; entry e in slot e % 3.  Two entries ahead of the one in use.
-    int j = next_tile(k_begin), j_next = j < k_end ? next_tile(j + kTile) : j;
-    long long r_cur = j < k_end ? key_row(j) : -1, r_next = j_next < k_end ? key_row(j_next) : -1;
-    int slot = 0;  // slot of K of the current tile
-    if (j < k_end) {
-      load(0, c.k, r_cur);
-      cp_async_commit();
-      load(1, c.v, r_cur);
+      const int row_n = un < units && jn < xn.k_end ? part_row(xn, jn) : 0;
+      if (j < x.k_end) {
+        load(&tk, row);
+        load(&tv, row);
+      }
+      if (head) {  // the unit's query rows (their place may still be in use: behind the first copies)
+        const int st = uq % QS, rows = min(8 * NT, R - x.row0);
+        bar_wait(&sm.dead, &sm.q_empty[st], ((uq / QS) & 1) ^ 1, a.err);
+        if (*reinterpret_cast<volatile int*>(&sm.dead)) break;
+        if (lane == 0) mbar_expect_tx(&sm.q_full[st], rows * Dh * 2);
+        __syncwarp();
+        if (lane < rows) {
+          const int r = x.row0 + lane, s = r / a.G;
+          bulk_g2s(sm.q[st][lane], a.q + (long long)(x.b * a.S + s) * a.q_ld + (long long)(x.kh * a.G + r - s * a.G) * Dh,
+                   Dh * 2, &sm.q_full[st], policy_evict_last());
+        }
+        ++uq;
+      }
+      head = un != u;
+      x = xn;
+      u = un;
+      j = jn;
+      row = row_n;
     }
-    cp_async_commit();
+    if (*reinterpret_cast<volatile int*>(&sm.dead)) {  // copies in flight end before the CTA does
+      for (int i = max(0, e - RING); i < e; ++i) mbar_wait_bounded(&sm.full[i % RING], (i / RING) & 1, a.err, 1u << 22);
+      for (int i = max(0, uq - QS); i < uq; ++i) mbar_wait_bounded(&sm.q_full[i % QS], (i / QS) & 1, a.err, 1u << 22);
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------------------- consumers
+  const int quad = lane & 3, oct = lane >> 2;
+  int e = 0, uq = 0;
+  for (int u = blockIdx.x; u < units; u += gridDim.x, ++uq) {
+    const DecodeUnit x = unit_at(u);
+    const int pos0 = x.len - a.S, set = uq & 1;
+    int prow[NT][2];  // positions of this lane's rows n = 8 t + 2 quad + i
     float m[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      m[t][0] = m[t][1] = kNone;
-      l[t][0] = l[t][1] = 0.0f;
 #pragma unroll
-      for (int x = 0; x < MT; ++x)
+      for (int i = 0; i < 2; ++i) {
+        const int r = x.row0 + 8 * t + 2 * quad + i;
+        prow[t][i] = r < R ? pos0 + r / a.G : -1;
+        m[t][i] = kNone;
+        l[t][i] = 0.0f;
+      }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[x][t][e] = 0.0f;
+      for (int y = 0; y < MT; ++y)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[y][t][i] = 0.0f;
     }
-    while (j < k_end) {
-      const int sv = slot + 1 == kRing ? 0 : slot + 1, sk2 = sv + 1 == kRing ? 0 : sv + 1;
-      cp_async_wait<1>();
-      __syncthreads();  // K has landed; the previous tile's V is free
-      if (j_next < k_end) load(sk2, c.k, r_next);
-      cp_async_commit();
-      // scores of this warp's 16 keys
+    bar_wait(&sm.dead, &sm.q_full[uq % QS], (uq / QS) & 1, a.err);
+    const uint32_t qbase = smem_u32(sm.q[uq % QS]) + (lane & 7) * (Dh + 8) * 2 + (lane >> 3) * 16;
+    for (int j = next_tile(x, x.k_begin); j < x.k_end; j = next_tile(x, j + kTile)) {
+      const int sk = e % RING, sv = (e + 1) % RING;
+      bar_wait(&sm.dead, &sm.full[sk], (e / RING) & 1, a.err);
       float s[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
+        for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
       {
         const int row = 16 * warp + (lane & 15);
-        const uint32_t base = smem_u32(sm.kv[slot]) + row * Dh * 2;
+        const uint32_t base = smem_u32(sm.kv[sk]) + row * 128;
 #pragma unroll
-        for (int k = 0; k < Dh / 16; ++k) {
-          uint32_t af[4];
-          ldsm_x4(af, base + (((2 * k + (lane >> 4)) ^ (row & 7)) << 4));
+        for (int k = 0; k < Dh / 32; ++k) {  // 32 dims: two K fragments, one load of query fragments per 8 rows
+          uint32_t k0[4], k1[4];
+          const uint32_t cbase = base + (k >> 1) * kTile * 128;
+          const int ch = (k & 1) * 4 + (lane >> 4);
+          ldsm_x4(k0, cbase + ((ch ^ (row & 7)) << 4));
+          ldsm_x4(k1, cbase + (((ch + 2) ^ (row & 7)) << 4));
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_bf16(s[t], af, qf[t][k][0], qf[t][k][1]);
+          for (int t = 0; t < NT; ++t) {
+            uint32_t qf[4];
+            ldsm_x4(qf, qbase + t * 8 * (Dh + 8) * 2 + k * 64);
+            mma_bf16(s[t], k0, qf[0], qf[1]);
+            mma_bf16(s[t], k1, qf[2], qf[3]);
+          }
         }
       }
-      const bool all = j + kTile - 1 <= pos0 && (a.vis.window == 0 || j >= a.vis.first(sl.len - 1));
-      float mn[NT][2];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[sk]);
+      const bool all = j + kTile - 1 <= pos0 && (a.vis.window == 0 || j >= a.vis.first(x.len - 1));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = j + 16 * warp + oct + 8 * (e >> 1);
-          s[t][e] = all || a.vis(prow[t][e & 1], key) ? __fmul_rn(s[t][e], a.scale2) : kNone;
+        for (int i = 0; i < 4; ++i) {
+          const int key = j + 16 * warp + oct + 8 * (i >> 1);
+          s[t][i] = all || a.vis(prow[t][i & 1], key) ? __fmul_rn(s[t][i], a.scale2) : kNone;
         }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(s[t][e], s[t][e + 2]);
+        for (int i = 0; i < 2; ++i) {
+          float v = fmaxf(s[t][i], s[t][i + 2]);
 #pragma unroll
-          for (int d = 4; d <= 16; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-          if (oct == 0) sm.mx[warp][8 * t + 2 * quad + e] = x;
+          for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+          if (oct == 0) sm.mx[warp][8 * t + 2 * quad + i] = v;
         }
       }
-      __syncthreads();  // K is free
+      consumers_sync();
       float alpha[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int n = 8 * t + 2 * quad + e;
-          mn[t][e] = fmaxf(fmaxf(m[t][e], fmaxf(sm.mx[0][n], sm.mx[1][n])), fmaxf(sm.mx[2][n], sm.mx[3][n]));
-          const float safe = mn[t][e] == kNone ? 0.0f : mn[t][e];  // nothing seen yet: every weight is 0
-          alpha[t][e] = ex2(__fsub_rn(m[t][e], safe));
-          m[t][e] = mn[t][e];
-          const float p0 = ex2(__fsub_rn(s[t][e], safe)), p1 = ex2(__fsub_rn(s[t][e + 2], safe));
-          l[t][e] = __fmaf_rn(l[t][e], alpha[t][e], __fadd_rn(p0, p1));
+        for (int i = 0; i < 2; ++i) {
+          const int n = 8 * t + 2 * quad + i;
+          const float mn =
+              fmaxf(fmaxf(m[t][i], fmaxf(sm.mx[0][n], sm.mx[1][n])), fmaxf(sm.mx[2][n], sm.mx[3][n]));
+          const float safe = mn == kNone ? 0.0f : mn;  // nothing seen yet: every weight is 0
+          alpha[t][i] = ex2(__fsub_rn(m[t][i], safe));
+          m[t][i] = mn;
+          const float p0 = ex2(__fsub_rn(s[t][i], safe)), p1 = ex2(__fsub_rn(s[t][i + 2], safe));
+          l[t][i] = __fmaf_rn(l[t][i], alpha[t][i], __fadd_rn(p0, p1));
           // the weights enter the second product as bf16 (relative error 2^-9 each, against the
           // output's own bf16 rounding of the same size); their sum l keeps all 32 bits
           sm.p[n][16 * warp + oct] = f2bf(p0);
           sm.p[n][16 * warp + oct + 8] = f2bf(p1);
         }
-      // V of the next tile goes where this tile's K was
-      if (j_next < k_end) load(slot, c.v, r_next);
-      cp_async_commit();
-      const int j_after = j_next < k_end ? next_tile(j_next + kTile) : j_next;
-      const long long r_after = j_after < k_end ? key_row(j_after) : -1;
-      cp_async_wait<2>();
-      __syncthreads();  // V and the weights have landed
+      bar_wait(&sm.dead, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
+      if (j + kTile > x.len || (a.vis.window != 0 && j < x.lo)) {
+        // values that no row sees may be anything, and their weight 0 has to stay 0: cleared
+        uint8_t* v = reinterpret_cast<uint8_t*>(sm.kv[sv]);
+        for (int i = tid; i < CB * kTile * 8; i += 128) {
+          const int key = j + ((i >> 3) & (kTile - 1));
+          if (key >= x.len || (a.vis.window != 0 && key < x.lo && key >= a.vis.sinks))
+            *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+      }
+      consumers_sync();
 #pragma unroll
-      for (int x = 0; x < MT; ++x)
+      for (int y = 0; y < MT; ++y)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[x][t][e] = __fmul_rn(o[x][t][e], alpha[t][e & 1]);
+          for (int i = 0; i < 4; ++i) o[y][t][i] = __fmul_rn(o[y][t][i], alpha[t][i & 1]);
       const uint32_t vbase = smem_u32(sm.kv[sv]);
 #pragma unroll
       for (int k = 0; k < kTile / 16; ++k) {
@@ -398,43 +482,42 @@ __global__ void __launch_bounds__(128, Dh == 256 ? 2 : 4) paged_decode_kernel(Pa
         }
         const int row = 16 * k + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-        for (int x = 0; x < MT; ++x) {
+        for (int y = 0; y < MT; ++y) {
           uint32_t vf[4];
-          const int ch = (warp * MT + x) * 2 + ((lane >> 3) & 1);
-          ldsm_x4_t(vf, vbase + row * Dh * 2 + ((ch ^ (row & 7)) << 4));
+          const int ch = (warp * MT + y) * 2 + ((lane >> 3) & 1);
+          ldsm_x4_t(vf, vbase + (ch >> 3) * kTile * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_bf16(o[x][t], vf, pf[t][0], pf[t][1]);
+          for (int t = 0; t < NT; ++t) mma_bf16(o[y][t], vf, pf[t][0], pf[t][1]);
         }
       }
-      j = j_next;
-      j_next = j_after;
-      r_next = r_after;
-      slot = sk2;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[sv]);
+      e += 2;
     }
-    cp_async_wait_all();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.q_empty[uq % QS]);
     // sums over the key lanes and warps; is the numerator finite?
-    bool odd = false;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int x = 0; x < MT; ++x)
+      for (int i = 0; i < 2; ++i) {
+        float v = l[t][i];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= !isfinite(o[x][t][e]);
+        for (int d = 4; d <= 16; d <<= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+        if (oct == 0) sm.sum[set][warp][8 * t + 2 * quad + i] = v;
+        bool odd = false;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = l[t][e];
-#pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) x = __fadd_rn(x, __shfl_xor_sync(0xFFFFFFFFu, x, d));
-        if (oct == 0) sm.sum[warp][8 * t + 2 * quad + e] = x;
+        for (int y = 0; y < MT; ++y) odd |= !isfinite(o[y][t][i]) || !isfinite(o[y][t][i + 2]);
+        if (odd && x.row0 + 8 * t + 2 * quad + i < R) sm.bad[set] = 1;
       }
-    }
-    odd = __syncthreads_or(odd);
-    const bool whole = sl.count == 1;  // the only slab: finish here
-    const long long part = (long long)b * a.max_slabs + i_slab;
+    consumers_sync();
+    const bool odd = sm.bad[set] != 0;
+    if (tid == 0) sm.bad[set ^ 1] = 0;
+    const long long part = (long long)x.b * a.max_slabs + x.part;
     auto store = [&](int r, int d, float val, float ll) {
-      const int s = r / a.G, h = kh * a.G + r - s * a.G;
-      if (whole) {
-        const long long t = b * a.S + s;
+      const int s = r / a.G, h = x.kh * a.G + r - s * a.G;
+      if (x.whole) {
+        const long long t = x.b * a.S + s;
         float y = ll == 0.0f ? 0.0f : __fdiv_rn(val, ll);
         if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[t * a.gate_ld + h * a.gate_hs + d])));
         a.out[(t * a.nq + h) * Dh + d] = f2bf(y);
@@ -446,100 +529,102 @@ __global__ void __launch_bounds__(128, Dh == 256 ? 2 : 4) paged_decode_kernel(Pa
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int n = 8 * t + 2 * quad + e, r = row0 + n;
+        for (int i = 0; i < 2; ++i) {
+          const int n = 8 * t + 2 * quad + i, r = x.row0 + n;
           if (r >= R) continue;
-          const float ll = __fadd_rn(__fadd_rn(sm.sum[0][n], sm.sum[1][n]), __fadd_rn(sm.sum[2][n], sm.sum[3][n]));
+          const float ll = __fadd_rn(__fadd_rn(sm.sum[set][0][n], sm.sum[set][1][n]),
+                                     __fadd_rn(sm.sum[set][2][n], sm.sum[set][3][n]));
 #pragma unroll
-          for (int x = 0; x < MT; ++x) {
-            const int d = (warp * MT + x) * 16 + oct;
-            store(r, d, o[x][t][e], ll);
-            store(r, d + 8, o[x][t][e + 2], ll);
+          for (int y = 0; y < MT; ++y) {
+            const int d = (warp * MT + y) * 16 + oct;
+            store(r, d, o[y][t][i], ll);
+            store(r, d + 8, o[y][t][i + 2], ll);
           }
-          if (!whole && warp == 0 && oct == 0) {
+          if (!x.whole && warp == 0 && oct == 0) {
             const int s = r / a.G;
-            a.ws_ml[(part * a.S + s) * a.nq + kh * a.G + r - s * a.G] = make_float2(m[t][e], ll);
+            a.ws_ml[(part * a.S + s) * a.nq + x.kh * a.G + r - s * a.G] = make_float2(m[t][i], ll);
           }
         }
+      __syncwarp();
     } else {
       // An infinity or NaN reached a sum: from a key that the row sees, or, as 0 * inf, from one it does not.
       // Settle it by the definition, a warp per row, reading visible keys only.
-      for (int n = warp; n < 8 * NT && row0 + n < R; n += 4) {
-        const int r = row0 + n, s = r / a.G, h = kh * a.G + r - s * a.G;
-        float mm = -INFINITY, ll = 0.0f, oo[Dh / 32] = {};
-        attend_row_strict<Dh>(c, a.q + (long long)(b * a.S + s) * a.q_ld + (long long)h * Dh, b, kh, pos0 + s, k_begin,
-                              k_end, a.vis, a.scale2, a.err, mm, ll, oo);
-        for (int e = 0; e < Dh / 32; ++e) store(r, lane * (Dh / 32) + e, oo[e], ll);
-        if (!whole && lane == 0) a.ws_ml[(part * a.S + s) * a.nq + h] = make_float2(mm, ll);
+      for (int n = warp; n < 8 * NT && x.row0 + n < R; n += 4) {
+        const int r = x.row0 + n, s = r / a.G, h = x.kh * a.G + r - s * a.G;
+        float mm = kNone, ll = 0.0f, oo[Dh / 32] = {};
+        attend_row_strict<Dh>(c, a.q + (long long)(x.b * a.S + s) * a.q_ld + (long long)h * Dh, x.b, x.kh, pos0 + s,
+                              x.k_begin, x.k_end, a.vis, a.scale2, a.err, mm, ll, oo);
+        for (int i = 0; i < Dh / 32; ++i) store(r, lane * (Dh / 32) + i, oo[i], ll);
+        if (!x.whole && lane == 0) a.ws_ml[(part * a.S + s) * a.nq + h] = make_float2(mm, ll);
       }
     }
-    __syncthreads();  // the shared buffers are free for the next unit
   }
 }
 
-// Joins the slabs of one (row, 64 dims): M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.  256
-// threads: 16 lanes of 4 dims x 16 groups, group g taking the slabs whose number is g mod 16, the groups'
-// sums added in order, so the order of additions belongs to the slabs' positions.
-template <int Dh>
+// Joins a row's slabs: M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.  A slab's class is its number mod
+// 16; every class is summed in order with its own running maximum, then the classes in order, so the
+// order of additions belongs to the slabs' positions, however the classes are dealt to threads.  A block takes
+// `4 * QB` dims of a row: QB lanes of 4 dims, 256 / QB groups of QB / 16 classes each.  QB = 16 when rows are few
+// (every class its own threads), Dh / 4 when there are enough rows to fill the GPU.
+template <int Dh, int QB>
 __global__ void __launch_bounds__(256) paged_join_kernel(PagedView c, DecodeArgs a) {
   pdl_trigger();
   pdl_wait();
-  __shared__ float s_m[8];
-  __shared__ float4 s_o[16][16];
-  __shared__ float s_l[16];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = tid >> 4, d_blk = (blockIdx.x % (Dh / 64)) * 64;
-  const int d = d_blk + (tid & 15) * 4, br = blockIdx.x / (Dh / 64);
+  constexpr int CPT = QB / 16, BPR = Dh / (4 * QB);  // classes per thread, blocks per row
+  __shared__ float4 s_o[16][QB];
+  __shared__ float2 s_ml[16];
+  const int tid = threadIdx.x, g = tid / QB, ln = tid - g * QB;
+  const int br = blockIdx.x / BPR, d0 = (blockIdx.x - br * BPR) * 4 * QB;
   const int rows = a.S * a.nq, b = br / rows, r = br - b * rows;  // r = s * nq + h
-  const SlabList sl = slab_list(c, a, b, nullptr);
+  const SlabList sl = slab_list(a, seq_len(c, b, nullptr));
   if (sl.count == 1) return;
   const float2* ml = a.ws_ml + (long long)b * a.max_slabs * rows + r;
-  const float* po = a.ws_o + ((long long)b * a.max_slabs * rows + r) * Dh + d;
-  float M = -INFINITY;
-  for (int i = tid; i < sl.count; i += 256) M = fmaxf(M, ml[(long long)i * rows].x);
+  const float* po = a.ws_o + ((long long)b * a.max_slabs * rows + r) * Dh + d0 + 4 * ln;
 #pragma unroll
-  for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, x));
-  if (lane == 0) s_m[warp] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
-  const float safe = M == -INFINITY ? 0.0f : M;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float den = 0.0f;
-  // listed slab i has number i (i < first) or from + i - first: begin each group at its residue
-  auto walk = [&](int i0, int i1, int shift) {
-    int i = i0 + ((g - (i0 + shift)) & 15);
+  for (int k = 0; k < CPT; ++k) {
+    const int cls = g * CPT + k;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, den = 0.0f;
+    // listed slab i has number i (i < first) or from + i - first: a class begins at its residue
+    auto walk = [&](int i0, int i1, int number0) {
 #pragma unroll 4
-    for (; i < i1; i += 16) {
-      const float2 v = ml[(long long)i * rows];
-      const float4 x = *reinterpret_cast<const float4*>(po + (long long)i * rows * Dh);
-      const float w = ex2(__fsub_rn(v.x, safe));
-      den = __fmaf_rn(w, v.y, den);
-      if (w != 0.0f) {  // a slab this row sees nothing of adds nothing
-        acc.x = __fmaf_rn(w, x.x, acc.x);
-        acc.y = __fmaf_rn(w, x.y, acc.y);
-        acc.z = __fmaf_rn(w, x.z, acc.z);
-        acc.w = __fmaf_rn(w, x.w, acc.w);
+      for (int i = i0 + ((cls - number0) & 15); i < i1; i += 16) {
+        const float2 v = ml[(long long)i * rows];
+        const float4 x = *reinterpret_cast<const float4*>(po + (long long)i * rows * Dh);
+        if (v.x == -INFINITY && v.y == 0.0f) continue;  // a slab this row sees nothing of
+        const float mn = fmaxf(M, v.x), safe = mn == -INFINITY ? 0.0f : mn;
+        const float w = ex2(__fsub_rn(v.x, safe)), f = ex2(__fsub_rn(M, safe));
+        M = mn;
+        den = __fmaf_rn(den, f, __fmul_rn(w, v.y));
+        acc.x = __fmaf_rn(acc.x, f, __fmul_rn(w, x.x));
+        acc.y = __fmaf_rn(acc.y, f, __fmul_rn(w, x.y));
+        acc.z = __fmaf_rn(acc.z, f, __fmul_rn(w, x.z));
+        acc.w = __fmaf_rn(acc.w, f, __fmul_rn(w, x.w));
       }
-    }
-  };
-  walk(0, sl.first, 0);
-  walk(sl.first, sl.count, sl.from - sl.first);
-  s_o[g][tid & 15] = acc;
-  if ((tid & 15) == 0) s_l[g] = den;
+    };
+    walk(0, sl.first, 0);
+    walk(sl.first, sl.count, sl.from);
+    s_o[cls][ln] = acc;
+    if (ln == 0) s_ml[cls] = make_float2(M, den);
+  }
   __syncthreads();
-  if (tid >= 64) return;
+  if (tid >= 4 * QB) return;
+  float M = -INFINITY, y = 0.0f, ll = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) M = fmaxf(M, s_ml[i].x);
+  const float safe = M == -INFINITY ? 0.0f : M;
   const float* so = reinterpret_cast<const float*>(s_o);
-  float y = 0.0f, ll = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    y = __fadd_rn(y, so[i * 64 + tid]);
-    ll = __fadd_rn(ll, s_l[i]);
+    const float f = ex2(__fsub_rn(s_ml[i].x, safe));
+    y = __fmaf_rn(f, so[i * 4 * QB + tid], y);
+    ll = __fmaf_rn(f, s_ml[i].y, ll);
   }
   y = ll == 0.0f ? 0.0f : __fdiv_rn(y, ll);
-  const int s = r / a.nq, h = r - s * a.nq, dd = d_blk + tid;
+  const int s = r / a.nq, h = r - s * a.nq, d = d0 + tid;
   const long long t = b * a.S + s;
-  if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[t * a.gate_ld + h * a.gate_hs + dd])));
-  a.out[(t * a.nq + h) * Dh + dd] = f2bf(y);
+  if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[t * a.gate_ld + h * a.gate_hs + d])));
+  a.out[(t * a.nq + h) * Dh + d] = f2bf(y);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -587,18 +672,26 @@ static size_t align_up(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <int Dh, int NT>
 static int launch_decode(const PagedView& v, const DecodeArgs& a, long long units, cudaStream_t st) {
-  const size_t smem = sizeof(DecodeSmem<Dh, NT>) + (v.B + 1) * sizeof(int);
+  constexpr size_t fixed = sizeof(DecodeSmem<Dh, NT>) + 1024;
   static DeviceOnce ready;
   if (!ready([] {
         return cudaFuncSetAttribute(paged_decode_kernel<Dh, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(sizeof(DecodeSmem<Dh, NT>) + (kMaxSeqs + 1) * sizeof(int)));
+                                    int(fixed + (2 * kMaxSeqs + 1) * sizeof(int)));
       }))
     return QMTP_ERR_CUDA;
-  const int per_sm = Dh == 256 ? 2 : 4;
-  const int grid = int(std::min<long long>(units, (long long)sm_count() * per_sm));
-  launch_kernel(paged_decode_kernel<Dh, NT>, dim3(grid), dim3(128), smem, st, v, a);
-  if (a.max_slabs > 1)
-    launch_kernel(paged_join_kernel<Dh>, dim3(v.B * a.S * a.nq * (Dh / 64)), dim3(256), 0, st, v, a);
+  CUtensorMap tk, tv;
+  const cuuint64_t kd[2] = {Dh, cuuint64_t((v.pages * v.nkv) << v.page_log)}, ks[1] = {Dh * 2};
+  const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kTile))};
+  if (!encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb)) return QMTP_ERR_CUDA;
+  const int grid = int(std::min<long long>(units, (long long)sm_count() * DecodeCfg<Dh>::per_sm));
+  launch_kernel(paged_decode_kernel<Dh, NT>, dim3(grid), dim3(160), fixed + (2 * v.B + 1) * sizeof(int), st, tk, tv, v, a);
+  if (a.max_slabs > 1) {
+    const int rows = v.B * a.S * a.nq;
+    if (rows >= 2 * sm_count())
+      launch_kernel(paged_join_kernel<Dh, Dh / 4>, dim3(rows), dim3(256), 0, st, v, a);
+    else
+      launch_kernel(paged_join_kernel<Dh, 16>, dim3(rows * (Dh / 64)), dim3(256), 0, st, v, a);
+  }
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
 }
 
@@ -681,7 +774,7 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   const bool two = S * G > 8;
   a.row_tiles = (S * G + (two ? 15 : 7)) / (two ? 16 : 8);
   const long long units = (long long)v.B * a.max_slabs * v.nkv * a.row_tiles;
-  if (units >= (1ll << 31) || (long long)v.B * S * a.nq >= (1ll << 28)) return QMTP_ERR_SHAPE;
+  if (units >= (1ll << 30) || (long long)v.B * S * a.nq >= (1ll << 28)) return QMTP_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define QMTP_DECODE(D) (two ? launch_decode<D, 2>(v, a, units, st) : launch_decode<D, 1>(v, a, units, st))
   return cache->Dh == 64 ? QMTP_DECODE(64) : cache->Dh == 128 ? QMTP_DECODE(128) : QMTP_DECODE(256);

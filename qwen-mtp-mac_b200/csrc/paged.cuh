@@ -91,6 +91,22 @@ __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t
   }
 }
 
+// A bounded barrier wait by every lane of a warp.  After one has run out (`dead`, in shared memory), every later
+// wait of the CTA returns at once, so that it ends soon; the error word tells.
+__device__ __forceinline__ void bar_wait(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
+  if (__any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile int*>(dead))) return;
+  if (!mbar_wait_bounded(bar, parity, err, 1u << 22)) *reinterpret_cast<volatile int*>(dead) = 1;
+  __syncwarp();
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // Runs a set-up call (a kernel's attributes) once for every device the process uses; false if it failed,
 // and a failure is tried again by the next call.
 struct DeviceOnce {
@@ -105,6 +121,17 @@ struct DeviceOnce {
     return true;
   }
 };
+
+// bf16 tensor map with 128-byte swizzle (boxes 64 elements wide); what lies outside reads as zeros.
+inline bool encode_pages(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                   const cuuint32_t* box) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return false;
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 // Host checks shared by the entry points; fills the device view.
 int paged_view(const qmtp_paged_cache* cache, PagedView* out);

@@ -54,13 +54,6 @@ struct PromptBars {
   int b, tile, n, c0, len;  // this CTA's sequence, row tile, new tokens, first row, length
 };
 
-// Every lane of the warp waits.
-__device__ __forceinline__ void bar_wait(PromptBars* s, uint64_t* bar, uint32_t parity, unsigned* err) {
-  if (__any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile int*>(&s->dead))) return;
-  if (!mbar_wait_bounded(bar, parity, err, 1u << 22)) *reinterpret_cast<volatile int*>(&s->dead) = 1;
-  __syncwarp();
-}
-
 // 128-byte swizzled operand tile: rows of 128 bytes in groups of 8 (1024 bytes).  K-major (Q, K): `sbo` is the group
 // stride, lbo unused; MN-major (V): lbo is the distance of the next 64 dims, sbo that of the next 8 keys.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -93,14 +86,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          smem_u32(dst)),
-      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-      : "memory");
-}
-
 template <int Dh>
 __global__ void __launch_bounds__(PromptCfg<Dh>::threads, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -207,7 +192,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
 #pragma unroll
         for (int h = 0; h < E; ++h) {
           const int e = pos * E + h, st = e % NS;
-          bar_wait(bars, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err);
+          bar_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err);
           if (*reinterpret_cast<volatile int*>(&bars->dead)) return;
           if (lane == 0) mbar_expect_tx(&bars->full[st], Cfg::entry);
           __syncwarp();
@@ -253,7 +238,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
 #pragma unroll
           for (int h = 0; h < E; ++h) {
             const int e = pos_k(t) * E + h, st = e % NS;
-            bar_wait(bars, &bars->full[st], (e / NS) & 1, a.err);
+            bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
             tc_fence_after();
             if (lane == 0) {
               const uint32_t qa = smem_u32(s_q + w * Cfg::q_bytes) + h * (CB / E) * kRows * 128;
@@ -276,7 +261,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           for (int h = 0; h < E; ++h) {
             constexpr int rows = kKeys / E;
             const int e = pos_v(t) * E + h, st = e % NS;
-            bar_wait(bars, &bars->full[st], (e / NS) & 1, a.err);
+            bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
             const int live = len - tile_key(t) - h * rows;  // rows of the entry that hold a key
             if (first && live < rows) {  // the sequence ends here: what lies behind may be anything, P = 0 must stay 0
               uint8_t* v = s_ring + st * Cfg::entry;
@@ -301,19 +286,19 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (lane == 0) umma_commit(t + 1 < nt ? &bars->pv[w] : &bars->done[w]);
           __syncwarp();
         };
-        bar_wait(bars, &bars->q_full, 0, a.err);
+        bar_wait(&bars->dead, &bars->q_full, 0, a.err);
         if (NQ == 1) {
           scores(0, 0, 0, true);
           for (int t = 0; t < nt; ++t) {
             if (t + 1 < nt) scores(0, t + 1, (t + 1) & 1, true);
-            bar_wait(bars, &bars->p_full[t & 1], (t >> 1) & 1, a.err);
+            bar_wait(&bars->dead, &bars->p_full[t & 1], (t >> 1) & 1, a.err);
             values(0, t, t & 1, true, true);
           }
         } else {
           for (int w = 0; w < chains; ++w) scores(w, 0, w, w == chains - 1);
           for (int t = 0; t < nt; ++t)
             for (int w = 0; w < chains; ++w) {
-              bar_wait(bars, &bars->p_full[w], t & 1, a.err);
+              bar_wait(&bars->dead, &bars->p_full[w], t & 1, a.err);
               values(w, t, w, w == 0, w == chains - 1);
               if (t + 1 < nt) scores(w, t + 1, w, w == chains - 1);
             }
@@ -334,7 +319,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       for (int t = 0; t < nt; ++t) {
         const int buf = NQ == 1 ? t & 1 : w, j0 = tile_key(t);
         const uint32_t t_s = tmem + lane_base + 256 + buf * kKeys;
-        bar_wait(bars, &bars->s_full[buf], NQ == 1 ? (t >> 1) & 1 : t & 1, a.err);
+        bar_wait(&bars->dead, &bars->s_full[buf], NQ == 1 ? (t >> 1) & 1 : t & 1, a.err);
         tc_fence_after();
         float s[kKeys];
 #pragma unroll
@@ -359,7 +344,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           const float alpha = mn == -INFINITY ? 1.0f : ex2(__fsub_rn(m, mn));
           m = mn;
           l = __fmul_rn(l, alpha);
-          bar_wait(bars, &bars->pv[w], (t - 1) & 1, a.err);
+          bar_wait(&bars->dead, &bars->pv[w], (t - 1) & 1, a.err);
           tc_fence_after();
 #pragma unroll 1
           for (int d = 0; d < Dh; d += 32) {
@@ -391,7 +376,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         mbar_arrive(&bars->p_full[buf]);
       }
       if (nt > 0) {
-        bar_wait(bars, &bars->done[w], 0, a.err);
+        bar_wait(&bars->dead, &bars->done[w], 0, a.err);
         tc_fence_after();
       }
       // O / l, gate, store; a row with an infinity or NaN is settled by the definition afterwards
@@ -508,16 +493,6 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedView c, PromptArg
 }
 
 // ----------------------------------------------------------------------------- host
-static bool encode(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
-                   const cuuint32_t* box) {
-  auto fn = tensor_map_encoder();
-  if (!fn) return false;
-  const cuuint32_t es[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // CTAs that a call needs at most (the sequences' row counts are only known on the device).
 static long long prompt_items(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
   const int NQ = c->Dh == 256 ? 1 : 2, TT = NQ * (kRows / (a->n_q / c->n_kv));
@@ -546,7 +521,7 @@ static int launch_prompt(const qmtp_paged_args* args, const PagedView& v, const 
   const cuuint32_t qb[3] = {64, cuuint32_t(a.G), cuuint32_t(a.tpt)};
   const cuuint64_t kd[2] = {Dh, cuuint64_t((v.pages * v.nkv) << v.page_log)}, ks[1] = {Dh * 2};
   const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kKeys / Cfg::E))};
-  if (!encode(&tq, a.q, 3, qd, qs, qb) || !encode(&tk, v.k, 2, kd, ks, kb) || !encode(&tv, v.v, 2, kd, ks, kb))
+  if (!encode_pages(&tq, a.q, 3, qd, qs, qb) || !encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb))
     return QMTP_ERR_CUDA;
   launch_kernel(paged_prompt_kernel<Dh>, dim3(unsigned(items), unsigned(a.splits)), dim3(Cfg::threads), Cfg::smem, st, tq, tk,
                 tv, v, a);

@@ -31,10 +31,13 @@ class PagedCache:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         _need(k.dim() == 4 and k.shape == v.shape, "k and v are [pages, n_kv, page, head_dim], of one shape")
-        _tensor("k", k, BF16, k.device)
-        _tensor("v", v, BF16, k.device)
+        self._k, self._v, self._index = k, v, k.get_device()
+        for name, t in (("k", k), ("v", v)):
+            _tensor(name, t, BF16, self._index)
         _lib.require_cuda(k, v)
-        self.k, self.v = k, v
+        self.pages, self.n_kv, self.page, self.head_dim = k.shape
+        self._base = bytes(_lib.PagedCacheArgs(k=k.data_ptr(), v=v.data_ptr(), pages=self.pages, n_kv=self.n_kv,
+                                               page=self.page, Dh=self.head_dim))
 
     @classmethod
     def empty(cls, pages: int, n_kv: int, head_dim: int, page: int = 64, device="cuda") -> "PagedCache":
@@ -43,30 +46,24 @@ class PagedCache:
         return cls(torch.empty(shape, dtype=BF16, device=device), torch.empty(shape, dtype=BF16, device=device))
 
     @property
-    def n_kv(self) -> int:
-        return self.k.shape[1]
+    def k(self) -> torch.Tensor:
+        return self._k
 
     @property
-    def page(self) -> int:
-        return self.k.shape[2]
-
-    @property
-    def head_dim(self) -> int:
-        return self.k.shape[3]
+    def v(self) -> torch.Tensor:
+        return self._v
 
     def _args(self, table: torch.Tensor, lens: torch.Tensor) -> "_lib.PagedCacheArgs":
-        dev = self.k.device
-        _tensor("table", table, torch.int32, dev)
-        _tensor("lens", lens, torch.int32, dev)
-        _need(table.dim() == 2 and lens.dim() == 1 and table.shape[0] == lens.shape[0],
-              "table is [sequences, pages of a sequence], lens [sequences]")
-        _need(table.shape[1] > 0 and table.stride(1) == 1 and lens.is_contiguous(), "table rows and lens need to be contiguous")
-        B, W = table.shape
-        ld = table.stride(0) if B > 1 else W
-        pages, n_kv, page, dh = self.k.shape
-        return _lib.PagedCacheArgs(k=self.k.data_ptr(), v=self.v.data_ptr(), table=table.data_ptr(),
-                                   lens=lens.data_ptr(), pages=pages, ld_table=ld, n_kv=n_kv, page=page, Dh=dh,
-                                   table_w=W, B=B)
+        _tensor("table", table, torch.int32, self._index)
+        _tensor("lens", lens, torch.int32, self._index)
+        if table.dim() != 2 or lens.dim() != 1:
+            _need(False, "table is [sequences, pages of a sequence], lens [sequences]")
+        (B, W), (ld, one) = table.shape, table.stride()
+        if lens.shape[0] != B or W == 0 or (one != 1 and W > 1) or not lens.is_contiguous():
+            _need(False, "table is [sequences, pages of a sequence] with contiguous rows, lens [sequences], contiguous")
+        a = _lib.PagedCacheArgs.from_buffer_copy(self._base)
+        a.table, a.lens, a.ld_table, a.table_w, a.B = table.data_ptr(), lens.data_ptr(), ld if B > 1 else W, W, B
+        return a
 
 
 def _need(ok: bool, what: str) -> None:
@@ -74,11 +71,25 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(f"qmtp.paged: {what}")
 
 
-def _tensor(name: str, t: torch.Tensor, dtype, device) -> None:
+def _tensor(name: str, t: torch.Tensor, dtype, index: int) -> None:
+    """t is a tensor of that type on the cache's device."""
+    if t.dtype is dtype and t.get_device() == index >= 0:
+        return
     if not t.is_cuda:
         raise RuntimeError("qmtp ops run on CUDA tensors only (no CPU fallback)")
     _need(t.dtype == dtype, f"{name} has type {t.dtype}, not {dtype}")
-    _need(t.device == device, f"{name} is on {t.device}, the cache on {device}")
+    _need(False, f"{name} is on {t.device}, the cache on cuda:{index}")
+
+
+def _call(index: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of the tensors' device, whichever device is current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
 def append_qkv(qkv, cache: PagedCache, table, lens, cu=None, *, n_heads: int, gated: bool = False, q_norm=None,
@@ -93,37 +104,42 @@ def append_qkv(qkv, cache: PagedCache, table, lens, cu=None, *, n_heads: int, ga
 
     -> (q bf16 [T, n_heads, head_dim], gate: a view [T, n_heads, head_dim] of qkv, or None).  Rows of no
     sequence, and rows at a negative position (lens[b] below the row count), are left as they were."""
-    dev, dh = cache.k.device, cache.head_dim
+    dev, dh = cache._index, cache.head_dim
     _tensor("qkv", qkv, BF16, dev)
-    _need(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv is [rows, width] with contiguous rows")
-    T, per = qkv.shape[0], 2 if gated else 1
-    width = (n_heads * per + 2 * cache.n_kv) * dh
-    _need(n_heads >= 1 and qkv.shape[1] >= width, f"a row of qkv needs {width} values")
-    B = table.shape[0]
-    _check_cu(cu, B, dev)
+    if qkv.dim() != 2 or qkv.stride(1) != 1:
+        _need(False, "qkv is [rows, width] with contiguous rows")
+    T, nq_width = qkv.shape[0], n_heads * (2 if gated else 1) * dh
+    width = nq_width + 2 * cache.n_kv * dh
+    if n_heads < 1 or qkv.shape[1] < width:
+        _need(False, f"a row of qkv needs {width} values")
+    _check_cu(cu, table.shape[0], dev)
     for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
         if w is not None:
             _tensor(name, w, BF16, dev)
-            _need(w.shape == (dh,) and w.is_contiguous(), f"{name} is [head_dim], contiguous")
-    _need((cos is None) == (sin is None), "cos and sin go together")
-    if cos is not None:
-        for name, t in (("cos", cos), ("sin", sin)):
-            _tensor(name, t, torch.float32, dev)
-            _need(t.dim() == 2 and t.shape == cos.shape and t.is_contiguous(), "cos and sin are [positions, rotary / 2], contiguous")
+            if w.shape != (dh,) or not w.is_contiguous():
+                _need(False, f"{name} is [head_dim], contiguous")
+    rotary = max_pos = 0
+    if cos is not None or sin is not None:
+        _need(cos is not None and sin is not None, "cos and sin go together")
+        _tensor("cos", cos, torch.float32, dev)
+        _tensor("sin", sin, torch.float32, dev)
+        if cos.dim() != 2 or sin.shape != cos.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+            _need(False, "cos and sin are [positions, rotary / 2], contiguous")
+        max_pos, rotary = cos.shape[0], 2 * cos.shape[1]
     if out is None:
-        out = torch.empty((T, n_heads, dh), dtype=BF16, device=dev)
+        out = qkv.new_empty((T, n_heads, dh))
     else:
         _tensor("out", out, BF16, dev)
         _need(out.shape == (T, n_heads, dh) and out.is_contiguous(), "out is [rows, n_heads, head_dim], contiguous")
-    gate = qkv[:, : n_heads * 2 * dh].unflatten(1, (n_heads, 2, dh))[:, :, 1] if gated else None
-    if T == 0:
-        return out, gate
-    args = cache._args(table, lens)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().qmtp_paged_append(
-            qkv.data_ptr(), _row_stride(qkv, width), T, _lib.ptr(cu), n_heads, int(gated), _lib.ptr(q_norm), _lib.ptr(k_norm),
-            float(eps), _lib.ptr(cos), _lib.ptr(sin), 0 if cos is None else 2 * cos.shape[1],
-            0 if cos is None else cos.shape[0], out.data_ptr(), ctypes.byref(args), _lib.stream()), "append_qkv")
+    gate = None
+    if gated:
+        ld = qkv.stride(0)
+        gate = qkv.as_strided((T, n_heads, dh), (ld, 2 * dh, 1), qkv.storage_offset() + dh)
+    if T:
+        ptr = _lib.ptr
+        _call(dev, "append_qkv", _lib.lib().qmtp_paged_append, qkv.data_ptr(), _row_stride(qkv, width), T, ptr(cu), n_heads,
+              1 if gated else 0, ptr(q_norm), ptr(k_norm), eps, ptr(cos), ptr(sin), rotary, max_pos, out.data_ptr(),
+              ctypes.byref(cache._args(table, lens)))
     return out, gate
 
 
@@ -132,31 +148,42 @@ def _row_stride(t, width: int) -> int:
     return t.stride(0) if t.shape[0] > 1 else -(-width // 8) * 8
 
 
-def _check_cu(cu, B: int, dev) -> None:
+def _check_cu(cu, B: int, dev: int) -> None:
     if cu is not None:
         _tensor("cu", cu, torch.int32, dev)
-        _need(cu.shape == (B + 1,) and cu.is_contiguous(), "cu is [sequences + 1], contiguous")
+        if cu.shape != (B + 1,) or not cu.is_contiguous():
+            _need(False, "cu is [sequences + 1], contiguous")
 
 
 def _attention_args(q, cache: PagedCache, gate, scale, window, sinks, out):
-    dev, dh = cache.k.device, cache.head_dim
+    dev, dh = cache._index, cache.head_dim
     _tensor("q", q, BF16, dev)
-    _need(q.dim() == 3 and q.shape[2] == dh, "q is [rows, heads, head_dim]")
-    T, nq, _ = q.shape
-    _need(nq >= 1 and q.stride(2) == 1 and (nq == 1 or q.stride(1) == dh), "a row of q needs to be contiguous")
+    if q.dim() != 3 or q.shape[2] != dh:
+        _need(False, "q is [rows, heads, head_dim]")
+    (T, nq, _), (_, hs, one) = q.shape, q.stride()
+    if nq < 1 or one != 1 or (hs != dh and nq > 1):
+        _need(False, "a row of q needs to be contiguous")
     if out is None:
-        out = torch.empty((T, nq * dh), dtype=BF16, device=dev)
+        out = q.new_empty((T, nq * dh))
     else:
         _tensor("out", out, BF16, dev)
         _need(out.shape == (T, nq * dh) and out.is_contiguous(), "out is [rows, heads * head_dim], contiguous")
-    a = _lib.PagedArgs(q=q.data_ptr(), gate=None, out=out.data_ptr(), q_ld=_row_stride(q, nq * dh), gate_ld=0, gate_hs=0,
-                       T=T, n_q=nq, scale=float(dh ** -0.5 if scale is None else scale), window=int(window),
-                       sinks=int(sinks))
+    a = _lib.PagedArgs(q.data_ptr(), None, out.data_ptr(), _row_stride(q, nq * dh), 0, 0, T, nq,
+                       dh ** -0.5 if scale is None else scale, window, sinks)
     if gate is not None:
         _tensor("gate", gate, BF16, dev)
-        _need(gate.shape == q.shape and gate.stride(2) == 1, "gate has q's shape and contiguous heads")
-        a.gate, a.gate_ld, a.gate_hs = gate.data_ptr(), gate.stride(0) if T > 1 else 0, gate.stride(1) if nq > 1 else 0
+        ld, hs, one = gate.stride() if gate.dim() == 3 else (0, 0, 0)
+        if gate.shape != q.shape or one != 1:
+            _need(False, "gate has q's shape and contiguous heads")
+        a.gate, a.gate_ld, a.gate_hs = gate.data_ptr(), ld if T > 1 else 0, hs if nq > 1 else 0
     return a, out
+
+
+def _launch(cache, what, fn, workspace, a, c, q, *args):
+    pa, pc = ctypes.byref(a), ctypes.byref(c)
+    n = workspace(pa, pc)
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    _call(cache._index, what, fn, pa, *args, pc, _lib.ptr(ws), n)
 
 
 def attention(q, cache: PagedCache, table, lens, *, gate=None, scale: float | None = None, window: int = 0,
@@ -169,15 +196,10 @@ def attention(q, cache: PagedCache, table, lens, *, gate=None, scale: float | No
     shape, any head and row strides): the result is multiplied by sigmoid(gate).  A token's result has the
     same bits whatever the batch, S and the page size are.  out must not overlap the inputs."""
     a, out = _attention_args(q, cache, gate, scale, window, sinks, out)
-    if q.shape[0] == 0:
-        return out
-    c = cache._args(table, lens)
-    L = _lib.lib()
-    with torch.cuda.device(cache.k.device):
-        n = L.qmtp_paged_attention_workspace(ctypes.byref(a), ctypes.byref(c))
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _lib.check(L.qmtp_paged_attention(ctypes.byref(a), ctypes.byref(c), _lib.ptr(ws), n, _lib.stream()),
-                   "paged attention")
+    if q.shape[0]:
+        L = _lib.lib()
+        _launch(cache, "paged attention", L.qmtp_paged_attention, L.qmtp_paged_attention_workspace, a,
+                cache._args(table, lens), q)
     return out
 
 
@@ -187,14 +209,9 @@ def prompt_attention(q, cache: PagedCache, table, lens, cu, *, gate=None, scale:
     last tokens of sequence b -> bf16 [T, heads * head_dim].  Masks, scale and gate as in ``attention``; rows of
     no sequence are left as they were.  Any number of new tokens per sequence; ``attention`` is the one for a few."""
     a, out = _attention_args(q, cache, gate, scale, window, sinks, out)
-    _check_cu(cu, table.shape[0], cache.k.device)
-    if q.shape[0] == 0:
-        return out
-    c = cache._args(table, lens)
-    L = _lib.lib()
-    with torch.cuda.device(cache.k.device):
-        n = L.qmtp_paged_prompt_workspace(ctypes.byref(a), ctypes.byref(c))
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _lib.check(L.qmtp_paged_prompt(ctypes.byref(a), cu.data_ptr(), ctypes.byref(c), _lib.ptr(ws), n, _lib.stream()),
-                   "paged prompt attention")
+    _check_cu(cu, table.shape[0], cache._index)
+    if q.shape[0]:
+        L = _lib.lib()
+        _launch(cache, "paged prompt attention", L.qmtp_paged_prompt, L.qmtp_paged_prompt_workspace, a,
+                cache._args(table, lens), q, cu.data_ptr())
     return out
