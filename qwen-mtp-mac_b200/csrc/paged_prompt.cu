@@ -28,6 +28,7 @@ struct PromptCfg {
   static constexpr int entry = kKeys * Dh * 2 / E;           // bytes
   static constexpr int stages = Dh == 64 ? 8 : 5;
   static constexpr int threads = NQ * 128 + 64;
+  static constexpr unsigned poly = Dh == 256 ? 0x22 : 0x52;  // of every 8 pairs of exponentials, those done by ex2_poly
   static constexpr int q_bytes = kRows * Dh * 2;
   static constexpr int smem = NQ * q_bytes + stages * entry + 1024 + 512;
 };
@@ -46,7 +47,7 @@ struct PromptArgs {
 };
 
 struct PromptBars {
-  uint64_t full[8], empty[8], q_full, s_full[2], p_full[2];
+  uint64_t full[8], empty[8], q_full, s_full[2], p_full[2][2];
   uint64_t pv[2];    // a phase per key tile but the last: O holds the products up to it
   uint64_t done[2];  // the last product
   uint32_t tmem;
@@ -81,6 +82,56 @@ __device__ __forceinline__ void tmem_ld32_ready(float* v) {
                  "+r"(u[16]), "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]),
                  "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])::"memory");
 }
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t x;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
+  return x != 0;
+}
+// Two fp32 values in a 64-bit register and the packed arithmetic on them.
+__device__ __forceinline__ uint64_t f2_pack(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^f on [-1/2, 1/2], degree 4: least squares at Chebyshev points, reweighted until the relative error was level, 2^-18.5
+constexpr float kE0 = 0.9999993f, kE1 = 0.6931218f, kE2 = 0.24024744f, kE3 = 0.05591786f, kE4 = 0.009570101f;
+// 2^x of a pair without the exponential unit, x <= 8; below 2^-126, and at -inf, 0.  x = n + f, |f| <= 1/2, by adding and
+// taking away 1.5 2^23; 2^f by the polynomial, n into the exponent bits.
+__device__ __forceinline__ void ex2_poly(uint64_t v, float& p0, float& p1) {
+  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f), unmagic = f2_pack(-12582912.0f, -12582912.0f);
+  const uint64_t minus = f2_pack(-1.0f, -1.0f);
+  const uint64_t r = f2_add(v, magic);
+  const uint64_t f = f2_fma(f2_add(r, unmagic), minus, v);
+  uint64_t p = f2_fma(f2_pack(kE4, kE4), f, f2_pack(kE3, kE3));
+  p = f2_fma(p, f, f2_pack(kE2, kE2));
+  p = f2_fma(p, f, f2_pack(kE1, kE1));
+  p = f2_fma(p, f, f2_pack(kE0, kE0));
+  float x0, x1, r0, r1;
+  f2_unpack(v, x0, x1);
+  f2_unpack(r, r0, r1);
+  f2_unpack(p, p0, p1);
+  p0 = x0 < -126.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+  p1 = x1 < -126.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -108,7 +159,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     mbar_init(&bars->q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->p_full[i], 128);
+      mbar_init(&bars->p_full[i][0], 128);
+      mbar_init(&bars->p_full[i][1], 128);
       mbar_init(&bars->pv[i], 1);
       mbar_init(&bars->done[i], 1);
     }
@@ -232,6 +284,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     } else if (warp == 4 * NQ + 1) {
       // ------------------------------------------------------------------ MMA
       if (nt > 0) {
+        const bool elected = elect_one();
         constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys);
         constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, Dh) | (1u << 16);  // B (V) is MN-major
         auto scores = [&](int w, int t, int buf, bool last) {  // S[buf] = Q_w K(t)^T
@@ -240,50 +293,52 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             const int e = pos_k(t) * E + h, st = e % NS;
             bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t qa = smem_u32(s_q + w * Cfg::q_bytes) + h * (CB / E) * kRows * 128;
-              const uint32_t ka = smem_u32(s_ring + st * Cfg::entry);
+            if (elected) {
+              const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes) + h * (CB / E) * kRows * 128, 16, 1024);
+              const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry), 16, 1024);
 #pragma unroll
               for (int k = 0; k < Dh / E / 16; ++k) {
-                const uint32_t off = (k >> 2) * kRows * 128 + (k & 3) * 32;
-                umma_bf16(tmem + 256 + buf * kKeys, desc_sw128(qa + off, 16, 1024), desc_sw128(ka + off, 16, 1024), idesc_s,
-                          (h | k) != 0);
+                const uint32_t off = ((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4;
+                umma_bf16(tmem + 256 + buf * kKeys, qd + off, kd + off, idesc_s, (h | k) != 0);
               }
               if (last) umma_commit(&bars->empty[st]);
             }
             __syncwarp();
           }
-          if (lane == 0) umma_commit(&bars->s_full[buf]);
+          if (elected) umma_commit(&bars->s_full[buf]);
           __syncwarp();
         };
-        auto values = [&](int w, int t, int buf, bool first, bool last) {  // O_w += P[buf] V(t)
+        auto values = [&](int w, int t, int buf, int parity, bool first, bool last) {  // O_w += P[buf] V(t)
 #pragma unroll
-          for (int h = 0; h < E; ++h) {
+          for (int hf = 0; hf < 2; ++hf) {  // halves of 64 keys, as the softmax hands them over
             constexpr int rows = kKeys / E;
-            const int e = pos_v(t) * E + h, st = e % NS;
-            bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
-            const int live = len - tile_key(t) - h * rows;  // rows of the entry that hold a key
-            if (first && live < rows) {  // the sequence ends here: what lies behind may be anything, P = 0 must stay 0
-              uint8_t* v = s_ring + st * Cfg::entry;
-              for (int i = lane; i < CB * rows * 8; i += 32) {
-                const int r = (i >> 3) % rows;
-                if (r >= live) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
+            const int e = pos_v(t) * E + (E == 2 ? hf : 0), st = e % NS;
+            if (E == 2 || hf == 0) {
+              bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+              const int live = len - tile_key(t) - (E == 2 ? hf * rows : 0);  // rows of the entry that hold a key
+              if (first && live < rows) {  // the sequence ends here: what lies behind may be anything, P = 0 must stay 0
+                uint8_t* v = s_ring + st * Cfg::entry;
+                for (int i = lane; i < CB * rows * 8; i += 32) {
+                  const int r = (i >> 3) % rows;
+                  if (r >= live) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();
+                __syncwarp();
               }
-              fence_proxy_async();
-              __syncwarp();
             }
+            bar_wait(&bars->dead, &bars->p_full[buf][hf], parity, a.err);
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t va = smem_u32(s_ring + st * Cfg::entry);
+            if (elected) {
+              const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + (E == 1 ? hf * 64 * 128 : 0), rows * 128, 1024);
 #pragma unroll
-              for (int k = 0; k < rows / 16; ++k)
-                umma_bf16_ts(tmem + w * Dh, tmem + 256 + buf * kKeys + h * (rows / 2) + k * 8,
-                             desc_sw128(va + k * 2048, rows * 128, 1024), idesc_o, t > 0 || (h | k) != 0);
-              if (last) umma_commit(&bars->empty[st]);
+              for (int k = 0; k < 4; ++k)
+                umma_bf16_ts(tmem + w * Dh, tmem + 256 + buf * kKeys + hf * 32 + k * 8, vd + k * (2048 >> 4), idesc_o,
+                             t > 0 || (hf | k) != 0);
+              if (last && (E == 2 || hf == 1)) umma_commit(&bars->empty[st]);
             }
             __syncwarp();
           }
-          if (lane == 0) umma_commit(t + 1 < nt ? &bars->pv[w] : &bars->done[w]);
+          if (elected) umma_commit(t + 1 < nt ? &bars->pv[w] : &bars->done[w]);
           __syncwarp();
         };
         bar_wait(&bars->dead, &bars->q_full, 0, a.err);
@@ -291,15 +346,13 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           scores(0, 0, 0, true);
           for (int t = 0; t < nt; ++t) {
             if (t + 1 < nt) scores(0, t + 1, (t + 1) & 1, true);
-            bar_wait(&bars->dead, &bars->p_full[t & 1], (t >> 1) & 1, a.err);
-            values(0, t, t & 1, true, true);
+            values(0, t, t & 1, (t >> 1) & 1, true, true);
           }
         } else {
           for (int w = 0; w < chains; ++w) scores(w, 0, w, w == chains - 1);
           for (int t = 0; t < nt; ++t)
             for (int w = 0; w < chains; ++w) {
-              bar_wait(&bars->dead, &bars->p_full[w], t & 1, a.err);
-              values(w, t, w, w == 0, w == chains - 1);
+              values(w, t, w, t & 1, w == 0, w == chains - 1);
               if (t + 1 < nt) scores(w, t + 1, w, w == chains - 1);
             }
         }
@@ -334,8 +387,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         }
         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 4; i < kKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-        const float top = __fmul_rn(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), a.scale2);
+        for (int i = 4; i < kKeys - 4; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
+        mx[0] = max3(mx[0], s[kKeys - 4], s[kKeys - 3]);
+        mx[1] = max3(mx[1], s[kKeys - 2], s[kKeys - 1]);
+        const float top = __fmul_rn(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), a.scale2);
         if (t == 0) {
           m = top;
         } else if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
@@ -358,22 +415,38 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           }
         }
         const float neg = m == -INFINITY ? 0.0f : -m;  // nothing seen yet: every weight is 0
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        uint32_t pk[kKeys / 2];
+        const uint64_t scale2 = f2_pack(a.scale2, a.scale2), neg2 = f2_pack(neg, neg);
+        uint64_t sum[2] = {0, 0};
+        // in halves of 64 keys, each handed over as soon as it is stored
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 2) {
-          const float x = ex2(__fmaf_rn(s[i], a.scale2, neg)), y = ex2(__fmaf_rn(s[i + 1], a.scale2, neg));
-          sum[i & 2] = __fadd_rn(sum[i & 2], x);
-          sum[(i & 2) + 1] = __fadd_rn(sum[(i & 2) + 1], y);
-          // bf16 weights: relative error 2^-9 each, of the size of the output's own rounding; l keeps fp32
-          pk[i / 2] = pack_bf16(x, y);
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t pk[kKeys / 4];
+#pragma unroll
+          for (int i = 0; i < kKeys / 4; ++i) {
+            const uint64_t v = f2_fma(f2_pack(s[hf * 64 + 2 * i], s[hf * 64 + 2 * i + 1]), scale2, neg2);
+            float x, y;
+            if ((Cfg::poly >> (i & 7)) & 1) {
+              ex2_poly(v, x, y);
+            } else {
+              f2_unpack(v, x, y);
+              x = ex2(x);
+              y = ex2(y);
+            }
+            sum[i & 1] = f2_add(sum[i & 1], f2_pack(x, y));
+            // bf16 weights: relative error 2^-9 each, of the size of the output's own rounding; l keeps fp32
+            pk[i] = pack_bf16(x, y);
+          }
+          tmem_st16(t_s + 32 * hf, pk);
+          tmem_st16(t_s + 32 * hf + 16, pk + 16);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&bars->p_full[buf][hf]);
         }
-        l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_st16(t_s + 16 * i, pk + 16 * i);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&bars->p_full[buf]);
+        {
+          float x, y;
+          f2_unpack(f2_add(sum[0], sum[1]), x, y);
+          l = __fadd_rn(l, __fadd_rn(x, y));
+        }
       }
       if (nt > 0) {
         bar_wait(&bars->dead, &bars->done[w], 0, a.err);
