@@ -305,8 +305,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     int e = 0, uq = 0;
     auto load = [&](const CUtensorMap* map, int row) {
       const int st = e % RING;
-      bar_wait(&sm.dead, &sm.empty[st], ((e / RING) & 1) ^ 1, a.err);
-      if (*reinterpret_cast<volatile int*>(&sm.dead)) return;
+      if (!warp_wait(&sm.dead, &sm.empty[st], ((e / RING) & 1) ^ 1, a.err)) return;
       if (lane == 0) mbar_expect_tx(&sm.full[st], kTile * Dh * 2);
       __syncwarp();
       const int r = __shfl_sync(0xFFFFFFFFu, row, min(part, parts - 1));
@@ -341,8 +340,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       }
       if (head) {  // the unit's query rows (their place may still be in use: behind the first copies)
         const int st = uq % QS, rows = min(8 * NT, R - x.row0);
-        bar_wait(&sm.dead, &sm.q_empty[st], ((uq / QS) & 1) ^ 1, a.err);
-        if (*reinterpret_cast<volatile int*>(&sm.dead)) break;
+        if (!warp_wait(&sm.dead, &sm.q_empty[st], ((uq / QS) & 1) ^ 1, a.err)) break;
         if (lane == 0) mbar_expect_tx(&sm.q_full[st], rows * Dh * 2);
         __syncwarp();
         if (lane < rows) {
@@ -387,11 +385,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[y][t][i] = 0.0f;
     }
-    bar_wait(&sm.dead, &sm.q_full[uq % QS], (uq / QS) & 1, a.err);
+    warp_wait(&sm.dead, &sm.q_full[uq % QS], (uq / QS) & 1, a.err);
     const uint32_t qbase = smem_u32(sm.q[uq % QS]) + (lane & 7) * (Dh + 8) * 2 + (lane >> 3) * 16;
     for (int j = next_tile(x, x.k_begin); j < x.k_end; j = next_tile(x, j + kTile)) {
       const int sk = e % RING, sv = (e + 1) % RING;
-      bar_wait(&sm.dead, &sm.full[sk], (e / RING) & 1, a.err);
+      warp_wait(&sm.dead, &sm.full[sk], (e / RING) & 1, a.err);
       float s[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -453,7 +451,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
           sm.p[n][16 * warp + oct] = f2bf(p0);
           sm.p[n][16 * warp + oct + 8] = f2bf(p1);
         }
-      bar_wait(&sm.dead, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
+      warp_wait(&sm.dead, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
       if (j + kTile > x.len || (a.vis.window != 0 && j < x.lo)) {
         // values that no row sees may be anything, and their weight 0 has to stay 0: cleared
         uint8_t* v = reinterpret_cast<uint8_t*>(sm.kv[sv]);

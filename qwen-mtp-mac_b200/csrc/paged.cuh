@@ -91,14 +91,29 @@ __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t
   }
 }
 
-// A bounded barrier wait by every lane of a warp.  After one has run out (`dead`, in shared memory), every later
-// wait of the CTA returns at once, so that it ends soon; the error word tells.
-__device__ __forceinline__ void bar_wait(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
-  if (__any_sync(0xFFFFFFFFu, *reinterpret_cast<volatile int*>(dead))) return;
-  if (!mbar_wait_bounded(bar, parity, err, 1u << 22)) *reinterpret_cast<volatile int*>(dead) = 1;
-  __syncwarp();
+// A bounded barrier wait.  Once one has run out (`dead`, in shared memory; the error word tells), the CTA's other
+// waits give up soon too.  False: gave up.
+__device__ __forceinline__ bool bar_wait_slow(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
+#pragma unroll 1
+  for (uint32_t it = 0; it < (1u << 22); ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(dead)) return false;
+  }
+  atomicOr(err, DEVERR_TIMEOUT);
+  *reinterpret_cast<volatile int*>(dead) = 1;
+  return false;
+}
+__device__ __forceinline__ bool bar_wait(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
+  return mbar_try_wait(bar, parity) || bar_wait_slow(dead, bar, parity, err);
+}
+// By every lane of a warp, which is converged afterwards.
+__device__ __forceinline__ bool warp_wait(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
+  return __all_sync(0xFFFFFFFFu, bar_wait(dead, bar, parity, err));
 }
 
+__device__ __forceinline__ void prefetch_tensormap(const void* tmap) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(

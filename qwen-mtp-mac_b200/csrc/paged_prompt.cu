@@ -1,16 +1,17 @@
 // Prompt attention over the paged cache on the tensor cores (tcgen05), for a ragged batch of chunks.
 //
-// A CTA owns NQ tiles of 128 query rows (128 / G tokens x the G query heads of a key head: all of them read
-// the same keys) and walks the key tiles (128 keys) they see with the running maximum m and sum l of the
+// A CTA per SM takes items of work in turn: NQ tiles of 128 query rows (128 / G tokens x the G query heads of a
+// key head: all of them read the same keys).  It walks the key tiles (128 keys) they see with the running maximum m and sum l of the
 // softmax.  Per key tile: S = Q K^T into TMEM; the tile's 128 threads, one row each, turn S into weights
 // P = 2^(S scale2 - m) in place (bf16); O += P V with P from TMEM.  O stays in TMEM and is rescaled only
 // when a row's maximum has grown by more than 2^kSlack since the last rescale, which leaves P <= 2^kSlack;
 // the final division by l takes it out again.
 //   warps 0 .. 4 NQ - 1   softmax, and at the end O / l, the gate and the store
-//   warp 4 NQ             TMA: pages into a ring of tiles (128-byte swizzle)
+//   warp 4 NQ             which item is next; TMA: pages into a ring of tiles (128-byte swizzle)
 //   warp 4 NQ + 1         MMA issue
-// Dh 256: one row tile, two S buffers (the scores of the next key tile run under this tile's softmax).
-// Dh 128, 64: two row tiles of one S buffer each, which take turns.  TMEM: O in columns [0, 256), S in [256, 512).
+// Each row tile has two score tiles in TMEM: the scores of the next keys run under this one's softmax.  Dh 256: one
+// row tile, 128 keys a score tile.  Dh 128, 64: two row tiles, 64 keys a score tile, where the tensor core and
+// the exponentials take about as long as each other.  TMEM: O in columns [0, 256), S in [256, 512).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -26,9 +27,9 @@ struct PromptCfg {
   static constexpr int NQ = Dh == 256 ? 1 : 2;               // row tiles per CTA
   static constexpr int E = Dh == 256 ? 2 : 1;                // ring entries per K or V tile (halves of 32 KB)
   static constexpr int entry = kKeys * Dh * 2 / E;           // bytes
+  static constexpr int SUB = kKeys / NQ;                     // keys of a score tile (two per row tile in TMEM)
   static constexpr int stages = Dh == 64 ? 8 : 5;
   static constexpr int threads = NQ * 128 + 64;
-  static constexpr unsigned poly = Dh == 256 ? 0x22 : 0x52;  // of every 8 pairs of exponentials, those done by ex2_poly
   static constexpr int q_bytes = kRows * Dh * 2;
   static constexpr int smem = NQ * q_bytes + stages * entry + 1024 + 512;
 };
@@ -46,13 +47,45 @@ struct PromptArgs {
   unsigned* err;
 };
 
+// One unit of work: a row tile (pair) of a sequence with one key head, and its share of the key tiles.
+struct PromptItem {
+  int b, kh, split, tok0, n, c0, len;  // b < 0: no more work
+};
+
 struct PromptBars {
-  uint64_t full[8], empty[8], q_full, s_full[2], p_full[2][2];
-  uint64_t pv[2];    // a phase per key tile but the last: O holds the products up to it
-  uint64_t done[2];  // the last product
+  uint64_t full[8], empty[8], q_full, q_empty, s_full[2][2], p_full[2][2][2];  // [row tile][score tile][64 keys]
+  uint64_t pv[2];    // a phase per score tile but an item's last: O holds the products up to it
+  uint64_t done[2];  // an item's last product
+  uint64_t item_full[2], item_empty[2], next_full;
+  alignas(16) uint4 next[1];
+  PromptItem item[2];
   uint32_t tmem;
-  int dead;   // a wait ran out: every later wait returns at once
-  int b, tile, n, c0, len;  // this CTA's sequence, row tile, new tokens, first row, length
+  int dead;  // a wait ran out: every later wait returns at once
+};
+
+// What an item's key tiles are, from its place.
+struct PromptTiles {
+  int p_first, p_last, chains, lo, lo_tile, sink_tiles, begin, nt, subs;
+  // SUB: keys of a score tile; subs: score tiles, without one that lies wholly behind the last row
+  __device__ __forceinline__ PromptTiles(const PromptItem& x, const PromptArgs& a, int NQ) {
+    const int SUB = kKeys / NQ;
+    p_first = x.len - x.n + x.tok0;
+    p_last = x.len - x.n + min(x.n, x.tok0 + NQ * a.tpt) - 1;
+    chains = NQ == 1 || x.tok0 + a.tpt >= x.n ? 1 : 2;  // row tiles that hold a token
+    // key tiles: [0, sink_tiles), then [lo / 128, p_last / 128]
+    lo = a.vis.first(max(p_first, 0));
+    lo_tile = lo / kKeys;
+    sink_tiles = a.vis.sinks > 0 && lo > 0 ? min((min(a.vis.sinks, lo) + kKeys - 1) / kKeys, lo_tile) : 0;
+    const int all = p_last < 0 ? 0 : sink_tiles + p_last / kKeys + 1 - lo_tile;
+    begin = int((long long)all * x.split / a.splits);
+    nt = int((long long)all * (x.split + 1) / a.splits) - begin;
+    subs = nt * NQ;
+    if (nt > 0 && key(nt - 1) + kKeys - SUB > p_last) --subs;
+  }
+  __device__ __forceinline__ int key(int t) const {  // first key of the t-th tile
+    t += begin;
+    return (t < sink_tiles ? t : lo_tile + t - sink_tiles) * kKeys;
+  }
 };
 
 // 128-byte swizzled operand tile: rows of 128 bytes in groups of 8 (1024 bytes).  K-major (Q, K): `sbo` is the group
@@ -82,6 +115,72 @@ __device__ __forceinline__ void tmem_ld32_ready(float* v) {
                  "+r"(u[16]), "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]),
                  "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])::"memory");
 }
+// Asks for a block of this grid that has not started: it will not start, and this block does its work.  The answer
+// (16 bytes) counts on `bar`.
+__device__ __forceinline__ void next_block_request(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The block's index in x, or -1: every block has started.
+__device__ __forceinline__ int next_block(const void* answer) {
+  uint32_t got, x = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\tld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n\t}"
+      : "=r"(got), "+r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  fence_proxy_async();
+  return got ? int(x) : -1;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max32(const float* s) {
+  float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+  for (int i = 4; i < 28; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
+  mx[0] = max3(mx[0], s[28], s[29]);
+  mx[1] = max3(mx[1], s[30], s[31]);
+  return fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+}
+// Bits [0, n) of a word, for any n.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; }
+// -inf for the scores of 32 keys that the row does not see: beyond hi, or before lw and not below sk.
+__device__ __forceinline__ void mask32(float* s, int hi, int lw, int sk) {
+  const uint32_t keep = below(hi + 1) & (~below(lw) | below(sk));
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!(keep >> i & 1)) s[i] = -INFINITY;
+}
+// 1 / (1 + e^-x) with the hardware's exponential and reciprocal (each within 2^-22)
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fadd_rn(1.0f, ex2(__fmul_rn(-kLog2e, x)))));
+  return y;
+}
+// Among four neighbouring lanes: lane q's v[j] becomes lane j's v[q].
+__device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
+#pragma unroll
+  for (int s = 1; s <= 2; s <<= 1) {
+    const bool up = (lane & s) != 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = s == 1 ? 2 * k : k, j = i + s;
+      const uint4 give = up ? v[i] : v[j];
+      const uint4 got = make_uint4(__shfl_xor_sync(0xFFFFFFFFu, give.x, s), __shfl_xor_sync(0xFFFFFFFFu, give.y, s),
+                                   __shfl_xor_sync(0xFFFFFFFFu, give.z, s), __shfl_xor_sync(0xFFFFFFFFu, give.w, s));
+      if (up) v[i] = got; else v[j] = got;
+    }
+  }
+}
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t x;
@@ -107,31 +206,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-// 2^f on [-1/2, 1/2], degree 4: least squares at Chebyshev points, reweighted until the relative error was level, 2^-18.5
-constexpr float kE0 = 0.9999993f, kE1 = 0.6931218f, kE2 = 0.24024744f, kE3 = 0.05591786f, kE4 = 0.009570101f;
-// 2^x of a pair without the exponential unit, x <= 8; below 2^-126, and at -inf, 0.  x = n + f, |f| <= 1/2, by adding and
-// taking away 1.5 2^23; 2^f by the polynomial, n into the exponent bits.
-__device__ __forceinline__ void ex2_poly(uint64_t v, float& p0, float& p1) {
-  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f), unmagic = f2_pack(-12582912.0f, -12582912.0f);
-  const uint64_t minus = f2_pack(-1.0f, -1.0f);
-  const uint64_t r = f2_add(v, magic);
-  const uint64_t f = f2_fma(f2_add(r, unmagic), minus, v);
-  uint64_t p = f2_fma(f2_pack(kE4, kE4), f, f2_pack(kE3, kE3));
-  p = f2_fma(p, f, f2_pack(kE2, kE2));
-  p = f2_fma(p, f, f2_pack(kE1, kE1));
-  p = f2_fma(p, f, f2_pack(kE0, kE0));
-  float x0, x1, r0, r1;
-  f2_unpack(v, x0, x1);
-  f2_unpack(r, r0, r1);
-  f2_unpack(p, p0, p1);
-  p0 = x0 < -126.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
-  p1 = x1 < -126.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -142,7 +216,7 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::threads, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, PagedView c, PromptArgs a) {
   using Cfg = PromptCfg<Dh>;
-  constexpr int NQ = Cfg::NQ, E = Cfg::E, NS = Cfg::stages, CB = Dh / 64;  // CB: 64-dim column blocks
+  constexpr int NQ = Cfg::NQ, E = Cfg::E, NS = Cfg::stages, SUB = Cfg::SUB, CB = Dh / 64;  // CB: 64-dim column blocks
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -150,258 +224,310 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   uint8_t* s_ring = base + NQ * Cfg::q_bytes;
   PromptBars* bars = reinterpret_cast<PromptBars*>(s_ring + NS * Cfg::entry);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int kh = blockIdx.x % c.nkv, item = blockIdx.x / c.nkv, split = blockIdx.y;
-  const int TT = NQ * a.tpt;  // tokens per CTA
 
   if (warp == 4 * NQ + 1) tmem_alloc(&bars->tmem, 512);
   if (warp == 4 * NQ && lane == 0) {
+    prefetch_tensormap(&tq);
+    prefetch_tensormap(&tk);
+    prefetch_tensormap(&tv);
     for (int i = 0; i < NS; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 1);
+    mbar_init(&bars->next_full, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->s_full[i], 1);
-      mbar_init(&bars->p_full[i][0], 128);
-      mbar_init(&bars->p_full[i][1], 128);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&bars->s_full[i][k], 1);
+        mbar_init(&bars->p_full[i][k][0], 128);
+        mbar_init(&bars->p_full[i][k][1], 128);
+      }
       mbar_init(&bars->pv[i], 1);
       mbar_init(&bars->done[i], 1);
+      mbar_init(&bars->item_full[i], 1);
+      mbar_init(&bars->item_empty[i], 4 * NQ + 1);
     }
     bars->dead = 0;
     fence_mbar_init();
   }
   pdl_wait();
-  if (warp == 0) {  // which sequence and row tile: the sequences' tiles counted a warp at a time
-    if (lane == 0) bars->b = -1;
-    __syncwarp();
-    int before = 0;
-    for (int i = 0; i < c.B; i += 32) {
-      const int k = i + lane;
-      int n = 0, c0 = 0;
-      if (k < c.B) {
-        c0 = a.cu[k];
-        const int c1 = a.cu[k + 1];
-        n = c1 - c0;
-        if (c0 < 0 || c1 > a.T || c1 < c0) {
-          if (blockIdx.x == 0) atomicOr(a.err, DEVERR_BADARG);
-          n = 0;
-        }
-      }
-      const int tiles = (n + TT - 1) / TT;
-      int incl = tiles;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int x = __shfl_up_sync(0xFFFFFFFFu, incl, d);
-        if (lane >= d) incl += x;
-      }
-      const int at = item - before - (incl - tiles);
-      if (at >= 0 && at < tiles) {
-        bars->b = k;
-        bars->tile = tiles - 1 - at;  // the last rows see the most keys: first
-        bars->n = n;
-        bars->c0 = c0;
-        bars->len = seq_len(c, k, a.err);
-      }
-      before += __shfl_sync(0xFFFFFFFFu, incl, 31);
-      if (item < before) break;
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
-  const int b = bars->b;
-  if (b >= 0) {
-    const int n = bars->n, len = bars->len, c0 = bars->c0, tok0 = bars->tile * TT;
-    const int p_first = len - n + tok0, p_last = len - n + min(n, tok0 + TT) - 1;
-    const int chains = NQ == 1 || tok0 + a.tpt >= n ? 1 : 2;  // row tiles that hold a token
-    // key tiles: [0, sink_tiles), then [lo / 128, p_last / 128]
-    const int lo = a.vis.first(max(p_first, 0)), lo_tile = lo / kKeys;
-    const int sink_tiles =
-        a.vis.sinks > 0 && lo > 0 ? min((min(a.vis.sinks, lo) + kKeys - 1) / kKeys, lo_tile) : 0;
-    const int nt_all = p_last < 0 ? 0 : sink_tiles + p_last / kKeys + 1 - lo_tile;
-    const int t_begin = int((long long)nt_all * split / a.splits), t_end = int((long long)nt_all * (split + 1) / a.splits);
-    const int nt = t_end - t_begin;
-    auto tile_key = [&](int t) {  // first key of the t-th tile of this CTA
-      t += t_begin;
-      return (t < sink_tiles ? t : lo_tile + t - sink_tiles) * kKeys;
-    };
-    // ring position of K(t), V(t): Dh 256 loads K0 K1 V0 K2 V1 ..., otherwise K0 V0 K1 V1 ...
-    auto pos_k = [&](int t) { return NQ == 1 ? (t == 0 ? 0 : 2 * t - 1) : 2 * t; };
-    auto pos_v = [&](int t) { return NQ == 1 ? min(2 * t + 2, 2 * nt - 1) : 2 * t + 1; };
+  // ring position, within an item, of K(t), V(t): Dh 256 loads K0 K1 V0 K2 V1 ..., otherwise K0 V0 K1 V1 ...
+  auto pos_k = [&](int t) { return NQ == 1 ? (t == 0 ? 0 : 2 * t - 1) : 2 * t; };
+  auto pos_v = [&](int t, int nt) { return NQ == 1 ? min(2 * t + 2, 2 * nt - 1) : 2 * t + 1; };
 
-    if (warp == 4 * NQ) {
-      // ------------------------------------------------------------------ TMA
-      const int box = min(1 << c.page_log, kKeys / E), parts = kKeys / box;  // rows per box, boxes down a tile
-      const long long none = (c.pages * c.nkv) << c.page_log;                // past the end: reads as zeros
-      // cache row of part `lane` of the tile at key j (a page that no row needs is not looked at)
-      auto part_row = [&](int j) -> int {
-        const int key = j + lane * box;
-        if (lane >= parts || key > p_last || (a.vis.window != 0 && key + box <= lo && key >= a.vis.sinks))
-          return int(none);
-        const long long r = cache_row(c, b, kh, key, a.err);
-        return int(r < 0 ? none : r);
-      };
-      int issued = 0;
-      auto load = [&](const CUtensorMap* map, int pos, bool is_v, int row) {
+  if (warp == 4 * NQ) {
+    // -------------------------------------------------------------------- items and TMA
+    const int TT = NQ * a.tpt;                                             // tokens per item
+    const int box = min(1 << c.page_log, kKeys / E), parts = kKeys / box;  // rows per box, boxes down a tile
+    const long long none = (c.pages * c.nkv) << c.page_log;                // past the end: reads as zeros
+    int seq = 0, before = 0;  // sequences [0, seq) hold `before` row tiles: items come in rising order
+    int e0 = 0, issued = 0, loads = 0;
+    long long u = blockIdx.x;
+    for (int i = 0;; ++i) {
+      // the next item: that of a block of the grid that has not started, taken over while this one runs
+      if (lane == 0) {
+        mbar_expect_tx(&bars->next_full, 16);
+        next_block_request(bars->next, &bars->next_full);
+      }
+      PromptItem x;
+      x.b = -1;
+      x.split = int(u % a.splits);
+      x.kh = int(u / a.splits % c.nkv);
+      const long long tile = u / a.splits / c.nkv;
+      while (seq < c.B) {
+        const int k = seq + lane;
+        int n = 0, c0 = 0, len = 0;
+        if (k < c.B) {
+          c0 = a.cu[k];
+          const int c1 = a.cu[k + 1];
+          len = seq_len(c, k, a.err);
+          n = c1 - c0;
+          if (c0 < 0 || c1 > a.T || c1 < c0) {
+            atomicOr(a.err, DEVERR_BADARG);
+            n = 0;
+          }
+        }
+        const int tiles = (n + TT - 1) / TT;
+        int incl = tiles;
 #pragma unroll
-        for (int h = 0; h < E; ++h) {
-          const int e = pos * E + h, st = e % NS;
-          bar_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err);
-          if (*reinterpret_cast<volatile int*>(&bars->dead)) return;
-          if (lane == 0) mbar_expect_tx(&bars->full[st], Cfg::entry);
-          __syncwarp();
-          issued = e + 1;
-          uint8_t* dst = s_ring + st * Cfg::entry;
-          // an entry: K all keys x half the dims, V half the keys x all dims (E == 2), else the whole tile
-          const int ncb = is_v ? CB : CB / E, np = is_v ? parts / E : parts, rows = is_v ? kKeys / E : kKeys;
-          const int part = lane / ncb, cb = lane - part * ncb;
-          const int r = __shfl_sync(0xFFFFFFFFu, row, (is_v ? h * np : 0) + min(part, np - 1));
-          if (part < np)
-            tma_load_2d(dst + cb * rows * 128 + part * box * 128, map, (is_v ? cb : h * ncb + cb) * 64, r, &bars->full[st],
-                        policy_evict_last());
+        for (int d = 1; d < 32; d <<= 1) {
+          const int y = __shfl_up_sync(0xFFFFFFFFu, incl, d);
+          if (lane >= d) incl += y;
         }
-      };
-      if (nt > 0) {
-        if (lane == 0) mbar_expect_tx(&bars->q_full, uint32_t(chains) * a.G * a.tpt * Dh * 2);
+        const long long at = tile - before - (incl - tiles);
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, at >= 0 && at < tiles);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          x.b = seq + src;
+          x.n = __shfl_sync(0xFFFFFFFFu, n, src);
+          x.c0 = __shfl_sync(0xFFFFFFFFu, c0, src);
+          x.len = __shfl_sync(0xFFFFFFFFu, len, src);
+          x.tok0 = (__shfl_sync(0xFFFFFFFFu, tiles, src) - 1 - int(__shfl_sync(0xFFFFFFFFu, int(at), src))) * TT;
+          break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, incl, 31);
+        seq += 32;
+      }
+      auto hand_out = [&](const PromptItem& y, int at) {
+        const bool ok = warp_wait(&bars->dead, &bars->item_empty[at & 1], ((at >> 1) & 1) ^ 1, a.err);
+        if (lane == 0) {
+          bars->item[at & 1] = y;
+          mbar_arrive(&bars->item_full[at & 1]);
+        }
         __syncwarp();
-        if (lane < chains * CB) {
-          const int w = lane / CB, cb = lane - w * CB;
-          tma_load_3d(s_q + w * Cfg::q_bytes + cb * kRows * 128, &tq, cb * 64, kh * a.G, c0 + tok0 + w * a.tpt, &bars->q_full);
-        }
-        int row = part_row(tile_key(0)), row_next = nt > 1 ? part_row(tile_key(1)) : 0;
+        return ok;
+      };
+      const bool ok = hand_out(x, i);
+      const PromptTiles ts(x, a, NQ);
+      if (ok && x.b >= 0 && ts.nt > 0) {
+        // cache row of part `lane` of the tile at key j (a page that no row needs is not looked at)
+        auto part_row = [&](int j) -> int {
+          const int key = j + lane * box;
+          if (lane >= parts || key > ts.p_last || (a.vis.window != 0 && key + box <= ts.lo && key >= a.vis.sinks))
+            return int(none);
+          const long long r = cache_row(c, x.b, x.kh, key, a.err);
+          return int(r < 0 ? none : r);
+        };
+        auto load = [&](const CUtensorMap* map, int pos, bool is_v, int row) {
+#pragma unroll
+          for (int h = 0; h < E; ++h) {
+            const int e = e0 + pos * E + h, st = e % NS;
+            if (!warp_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err)) return;
+            if (lane == 0) mbar_expect_tx(&bars->full[st], Cfg::entry);
+            __syncwarp();
+            issued = e + 1;
+            uint8_t* dst = s_ring + st * Cfg::entry;
+            // an entry: K all keys x half the dims, V half the keys x all dims (E == 2), else the whole tile
+            const int ncb = is_v ? CB : CB / E, np = is_v ? parts / E : parts, rows = is_v ? kKeys / E : kKeys;
+            const int part = lane / ncb, cb = lane - part * ncb;
+            const int r = __shfl_sync(0xFFFFFFFFu, row, (is_v ? h * np : 0) + min(part, np - 1));
+            if (part < np)
+              tma_load_2d(dst + cb * rows * 128 + part * box * 128, map, (is_v ? cb : h * ncb + cb) * 64, r, &bars->full[st],
+                          policy_evict_last());
+          }
+        };
+        auto load_q = [&] {
+          if (!warp_wait(&bars->dead, &bars->q_empty, (loads & 1) ^ 1, a.err)) return;
+          if (lane == 0) mbar_expect_tx(&bars->q_full, uint32_t(ts.chains) * a.G * a.tpt * Dh * 2);
+          __syncwarp();
+          if (lane < ts.chains * CB) {
+            const int w = lane / CB, cb = lane - w * CB;
+            tma_load_3d(s_q + w * Cfg::q_bytes + cb * kRows * 128, &tq, cb * 64, x.kh * a.G, x.c0 + x.tok0 + w * a.tpt,
+                        &bars->q_full);
+          }
+          ++loads;
+        };
+        const bool first = loads == 0;
+        if (first) load_q();  // later its place is still in use: behind the first keys
+        int row = part_row(ts.key(0)), row_next = ts.nt > 1 ? part_row(ts.key(1)) : 0;
         load(&tk, pos_k(0), false, row);
-        for (int t = 0; t < nt; ++t) {
-          const int row_after = t + 2 < nt ? part_row(tile_key(t + 2)) : 0;
-          if (NQ == 2) load(&tv, pos_v(t), true, row);
-          if (t + 1 < nt) load(&tk, pos_k(t + 1), false, row_next);
-          if (NQ == 1) load(&tv, pos_v(t), true, row);
+        if (!first) load_q();
+        for (int t = 0; t < ts.nt; ++t) {
+          const int row_after = t + 2 < ts.nt ? part_row(ts.key(t + 2)) : 0;
+          if (NQ == 2) load(&tv, pos_v(t, ts.nt), true, row);
+          if (t + 1 < ts.nt) load(&tk, pos_k(t + 1), false, row_next);
+          if (NQ == 1) load(&tv, pos_v(t, ts.nt), true, row);
           row = row_next;
           row_next = row_after;
         }
-        if (*reinterpret_cast<volatile int*>(&bars->dead)) {  // copies in flight end before the CTA does
-          mbar_wait_bounded(&bars->q_full, 0, a.err, 1u << 22);
-          for (int e = max(0, issued - NS); e < issued; ++e) mbar_wait_bounded(&bars->full[e % NS], (e / NS) & 1, a.err, 1u << 22);
-        }
+        e0 += 2 * ts.nt * E;
       }
-    } else if (warp == 4 * NQ + 1) {
-      // ------------------------------------------------------------------ MMA
-      if (nt > 0) {
-        const bool elected = elect_one();
-        constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, kKeys);
-        constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, Dh) | (1u << 16);  // B (V) is MN-major
-        auto scores = [&](int w, int t, int buf, bool last) {  // S[buf] = Q_w K(t)^T
+      int next = -1;
+      if (bar_wait(&bars->dead, &bars->next_full, i & 1, a.err)) next = next_block(bars->next);
+      next = __shfl_sync(0xFFFFFFFFu, next, 0);
+      if (x.b < 0 || !ok) break;
+      if (next < 0) {
+        x.b = -1;
+        hand_out(x, i + 1);
+        break;
+      }
+      u = next;
+    }
+    if (*reinterpret_cast<volatile int*>(&bars->dead)) {  // copies in flight end before the CTA does
+      if (loads > 0) mbar_wait_bounded(&bars->q_full, (loads - 1) & 1, a.err, 1u << 22);
+      for (int e = max(0, issued - NS); e < issued; ++e)
+        mbar_wait_bounded(&bars->full[e % NS], (e / NS) & 1, a.err, 1u << 22);
+    }
+  } else if (warp == 4 * NQ + 1) {
+    // -------------------------------------------------------------------- MMA
+    if (elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, Cfg::SUB);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, Dh) | (1u << 16);  // B (V) is MN-major
+      int e0 = 0, items = 0, work = 0;
+      int g[2] = {0, 0};  // score tiles so far, per row tile
+      int finished[2] = {0, 0};
+      for (;; ++items) {
+        if (!bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)) break;
+        const PromptItem x = bars->item[items & 1];
+        mbar_arrive(&bars->item_empty[items & 1]);
+        if (x.b < 0) break;
+        const PromptTiles ts(x, a, NQ);
+        const int nt = ts.nt;
+        if (nt == 0) continue;
+        const int subs = ts.subs;
+        auto scores = [&](int w, int j, bool last) {  // S = Q_w K^T of score tile j
+          const int buf = (g[w] + j) & 1, t = j / NQ, r0 = (j - t * NQ) * Cfg::SUB;
 #pragma unroll
           for (int h = 0; h < E; ++h) {
-            const int e = pos_k(t) * E + h, st = e % NS;
+            const int e = e0 + pos_k(t) * E + h, st = e % NS;
             bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
             tc_fence_after();
-            if (elected) {
-              const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes) + h * (CB / E) * kRows * 128, 16, 1024);
-              const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry), 16, 1024);
+            const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes) + h * (CB / E) * kRows * 128, 16, 1024);
+            const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, 16, 1024);
 #pragma unroll
-              for (int k = 0; k < Dh / E / 16; ++k) {
-                const uint32_t off = ((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4;
-                umma_bf16(tmem + 256 + buf * kKeys, qd + off, kd + off, idesc_s, (h | k) != 0);
-              }
-              if (last) umma_commit(&bars->empty[st]);
+            for (int k = 0; k < Dh / E / 16; ++k) {
+              const uint32_t off = ((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4;
+              umma_bf16(tmem + 256 + (2 * w + buf) * Cfg::SUB, qd + off, kd + off, idesc_s, (h | k) != 0);
             }
-            __syncwarp();
+            if (last && (j % NQ == NQ - 1 || j + 1 == subs)) umma_commit(&bars->empty[st]);
+            if (last && j + 1 == subs && h + 1 == E) umma_commit(&bars->q_empty);
           }
-          if (elected) umma_commit(&bars->s_full[buf]);
-          __syncwarp();
+          umma_commit(&bars->s_full[w][buf]);
         };
-        auto values = [&](int w, int t, int buf, int parity, bool first, bool last) {  // O_w += P[buf] V(t)
+        auto values = [&](int w, int j, bool last) {  // O_w += P V of score tile j
+          const int buf = (g[w] + j) & 1, parity = ((g[w] + j) >> 1) & 1, t = j / NQ, r0 = (j - t * NQ) * Cfg::SUB;
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {  // halves of 64 keys, as the softmax hands them over
+          for (int hf = 0; hf < Cfg::SUB / 64; ++hf) {  // 64 keys, as the softmax hands them over
             constexpr int rows = kKeys / E;
-            const int e = pos_v(t) * E + (E == 2 ? hf : 0), st = e % NS;
-            if (E == 2 || hf == 0) {
-              bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
-              const int live = len - tile_key(t) - (E == 2 ? hf * rows : 0);  // rows of the entry that hold a key
-              if (first && live < rows) {  // the sequence ends here: what lies behind may be anything, P = 0 must stay 0
-                uint8_t* v = s_ring + st * Cfg::entry;
-                for (int i = lane; i < CB * rows * 8; i += 32) {
-                  const int r = (i >> 3) % rows;
-                  if (r >= live) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_proxy_async();
-                __syncwarp();
-              }
-            }
-            bar_wait(&bars->dead, &bars->p_full[buf][hf], parity, a.err);
+            const int e = e0 + pos_v(t, nt) * E + hf, st = e % NS;
+            bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+            bar_wait(&bars->dead, &bars->p_full[w][buf][hf], parity, a.err);
             tc_fence_after();
-            if (elected) {
-              const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + (E == 1 ? hf * 64 * 128 : 0), rows * 128, 1024);
+            const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, rows * 128, 1024);
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_bf16_ts(tmem + w * Dh, tmem + 256 + buf * kKeys + hf * 32 + k * 8, vd + k * (2048 >> 4), idesc_o,
-                             t > 0 || (hf | k) != 0);
-              if (last && (E == 2 || hf == 1)) umma_commit(&bars->empty[st]);
-            }
-            __syncwarp();
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_ts(tmem + w * Dh, tmem + 256 + (2 * w + buf) * Cfg::SUB + hf * 32 + k * 8, vd + k * (2048 >> 4),
+                           idesc_o, j > 0 || (hf | k) != 0);
+            if (last && (j % NQ == NQ - 1 || j + 1 == subs)) umma_commit(&bars->empty[st]);
           }
-          if (elected) umma_commit(t + 1 < nt ? &bars->pv[w] : &bars->done[w]);
-          __syncwarp();
+          umma_commit(j + 1 < subs ? &bars->pv[w] : &bars->done[w]);
         };
-        bar_wait(&bars->dead, &bars->q_full, 0, a.err);
-        if (NQ == 1) {
-          scores(0, 0, 0, true);
-          for (int t = 0; t < nt; ++t) {
-            if (t + 1 < nt) scores(0, t + 1, (t + 1) & 1, true);
-            values(0, t, t & 1, (t >> 1) & 1, true, true);
-          }
-        } else {
-          for (int w = 0; w < chains; ++w) scores(w, 0, w, w == chains - 1);
-          for (int t = 0; t < nt; ++t)
-            for (int w = 0; w < chains; ++w) {
-              values(w, t, w, t & 1, w == 0, w == chains - 1);
-              if (t + 1 < nt) scores(w, t + 1, w, w == chains - 1);
-            }
+        bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
+        ++work;
+        for (int w = 0; w < ts.chains; ++w) scores(w, 0, w == ts.chains - 1);
+        for (int j = 0; j < subs; ++j) {
+          if (j + 1 < subs)
+            for (int w = 0; w < ts.chains; ++w) scores(w, j + 1, w == ts.chains - 1);
+          for (int w = 0; w < ts.chains; ++w) values(w, j, w == ts.chains - 1);
         }
-        for (int w = 0; w < chains; ++w) mbar_wait_bounded(&bars->done[w], 0, a.err, 1u << 22);
-        __syncwarp();
+        e0 += 2 * nt * E;
+        for (int w = 0; w < ts.chains; ++w) { g[w] += subs; ++finished[w]; }
       }
-    } else if (warp / 4 < chains) {
-      // ------------------------------------------------------------------ softmax: thread = row
-      const int w = warp >> 2, r = tid & 127;
-      const int i_tok = tok0 + w * a.tpt + r / a.G;  // token of the chunk
-      const bool valid = r < a.G * a.tpt && i_tok < n;
-      const int h = kh * a.G + r % a.G, p = len - n + i_tok;
-      const int pw0 = len - n + tok0 + w * a.tpt, pw1 = min(len - 1, pw0 + a.tpt - 1);  // the row tile's positions
-      const uint32_t lane_base = uint32_t(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in bits 16..
-      const uint32_t t_o = tmem + lane_base + w * Dh;
+      // every product is over before the tensor memory is given back
+      for (int w = 0; w < NQ; ++w)
+        if (finished[w] > 0) mbar_wait_bounded(&bars->done[w], (finished[w] - 1) & 1, a.err, 1u << 22);
+    }
+    __syncwarp();
+  } else if (warp < 4 * NQ) {
+    // -------------------------------------------------------------------- softmax: thread = row
+    const int w = warp >> 2, r = tid & 127;
+    const uint32_t lane_base = uint32_t(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in bits 16..
+    const uint32_t t_o = tmem + lane_base + w * Dh;
+    int g = 0, pvs = 0, finished = 0;  // score tiles, phases of pv and of done so far
+    int e0 = 0;                        // ring entries of the items so far
+    for (int items = 0;; ++items) {
+      if (!warp_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)) break;
+      const PromptItem x = bars->item[items & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->item_empty[items & 1]);
+      if (x.b < 0) break;
+      const PromptTiles ts(x, a, NQ);
+      const int e_item = e0;
+      e0 += 2 * ts.nt * E;
+      if (w >= ts.chains) continue;
+      const int nt = ts.nt, i_tok = x.tok0 + w * a.tpt + r / a.G;  // token of the chunk
+      const bool valid = r < a.G * a.tpt && i_tok < x.n;
+      const int h = x.kh * a.G + r % a.G, p = x.len - x.n + i_tok;
+      const int pw0 = x.len - x.n + x.tok0 + w * a.tpt, pw1 = min(x.len - 1, pw0 + a.tpt - 1);  // the row tile's positions
       float m = -INFINITY, l = 0.0f;  // m: maximum in use, in units of scale2
-      for (int t = 0; t < nt; ++t) {
-        const int buf = NQ == 1 ? t & 1 : w, j0 = tile_key(t);
-        const uint32_t t_s = tmem + lane_base + 256 + buf * kKeys;
-        bar_wait(&bars->dead, &bars->s_full[buf], NQ == 1 ? (t >> 1) & 1 : t & 1, a.err);
+      for (int j = 0; j < ts.subs; ++j) {
+        const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, j0 = ts.key(t) + r0;
+        const uint32_t t_s = tmem + lane_base + 256 + (2 * w + buf) * SUB;
+        warp_wait(&bars->dead, &bars->s_full[w][buf], ((g + j) >> 1) & 1, a.err);
         tc_fence_after();
-        float s[kKeys];
+        float s[SUB];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_nowait(t_s + 32 * i, s + 32 * i);
+        for (int i = 0; i < SUB; i += 32) tmem_ld32_nowait(t_s + i, s + i);
+        if (j0 + SUB > x.len) {
+          // The sequence ends in this tile: the values behind its end may be anything, and their weight 0 has to stay
+          // 0.  They are cleared before the weights are handed over.
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32_ready(s + 32 * i);
-        if (j0 + kKeys - 1 > pw0 || (a.vis.window != 0 && j0 < a.vis.first(pw1))) {
+          for (int k = 0; k < E; ++k) {
+            constexpr int rows = SUB / E;
+            const int e = e_item + pos_v(t, nt) * E + k, st = e % NS;
+            warp_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+            for (int i = r; i < CB * rows * 8; i += 128) {
+              const int row = (i >> 3) % rows, cb = (i >> 3) / rows;
+              if (j0 + k * rows + row >= x.len)
+                *reinterpret_cast<uint4*>(s_ring + st * Cfg::entry + ((cb * (kKeys / E) + r0 + row) * 8 + (i & 7)) * 16) =
+                    make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < SUB; i += 32) tmem_ld32_ready(s + i);
+        if (j0 + SUB - 1 > pw0 || (a.vis.window != 0 && j0 < a.vis.first(pw1))) {
           const int hi = p - j0, lw = a.vis.first(p) - j0, sk = a.vis.sinks - j0;
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (i > hi || (i < lw && i >= sk)) s[i] = -INFINITY;
+          for (int i = 0; i < SUB; i += 32) mask32(s + i, hi - i, lw - i, sk - i);
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
+        float top = max32(s);
 #pragma unroll
-        for (int i = 4; i < kKeys - 4; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], s[i + 2 * k], s[i + 2 * k + 1]);
-        mx[0] = max3(mx[0], s[kKeys - 4], s[kKeys - 3]);
-        mx[1] = max3(mx[1], s[kKeys - 2], s[kKeys - 1]);
-        const float top = __fmul_rn(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), a.scale2);
-        if (t == 0) {
+        for (int i = 32; i < SUB; i += 32) top = fmaxf(top, max32(s + i));
+        top = __fmul_rn(top, a.scale2);
+        if (j == 0) {
           m = top;
         } else if (__any_sync(0xFFFFFFFFu, top > m + kSlack)) {
-          // O is complete once the products up to tile t - 1 are (S of tile t implies those up to t - 2)
+          // O is complete once the products up to tile j - 1 are (S of tile j implies those up to j - 2)
           const float mn = top > m + kSlack ? top : m;
           const float alpha = mn == -INFINITY ? 1.0f : ex2(__fsub_rn(m, mn));
           m = mn;
           l = __fmul_rn(l, alpha);
-          bar_wait(&bars->dead, &bars->pv[w], (t - 1) & 1, a.err);
+          warp_wait(&bars->dead, &bars->pv[w], (pvs + j - 1) & 1, a.err);
           tc_fence_after();
 #pragma unroll 1
           for (int d = 0; d < Dh; d += 32) {
@@ -417,109 +543,136 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const float neg = m == -INFINITY ? 0.0f : -m;  // nothing seen yet: every weight is 0
         const uint64_t scale2 = f2_pack(a.scale2, a.scale2), neg2 = f2_pack(neg, neg);
         uint64_t sum[2] = {0, 0};
-        // in halves of 64 keys, each handed over as soon as it is stored
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t pk[kKeys / 4];
+        for (int c = 0; c < SUB / 32; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < kKeys / 4; ++i) {
-            const uint64_t v = f2_fma(f2_pack(s[hf * 64 + 2 * i], s[hf * 64 + 2 * i + 1]), scale2, neg2);
+          for (int i = 0; i < 16; ++i) {
             float x, y;
-            if ((Cfg::poly >> (i & 7)) & 1) {
-              ex2_poly(v, x, y);
-            } else {
-              f2_unpack(v, x, y);
-              x = ex2(x);
-              y = ex2(y);
-            }
+            f2_unpack(f2_fma(f2_pack(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), scale2, neg2), x, y);
+            x = ex2(x);
+            y = ex2(y);
             sum[i & 1] = f2_add(sum[i & 1], f2_pack(x, y));
             // bf16 weights: relative error 2^-9 each, of the size of the output's own rounding; l keeps fp32
             pk[i] = pack_bf16(x, y);
           }
-          tmem_st16(t_s + 32 * hf, pk);
-          tmem_st16(t_s + 32 * hf + 16, pk + 16);
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&bars->p_full[buf][hf]);
+          tmem_st16(t_s + 16 * c, pk);
+          if (c & 1) {  // 64 keys are handed over as soon as they are stored
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&bars->p_full[w][buf][c >> 1]);
+          }
         }
-        {
-          float x, y;
-          f2_unpack(f2_add(sum[0], sum[1]), x, y);
-          l = __fadd_rn(l, __fadd_rn(x, y));
-        }
+        float x, y;
+        f2_unpack(f2_add(sum[0], sum[1]), x, y);
+        l = __fadd_rn(l, __fadd_rn(x, y));
       }
+      // Four lanes share their rows' stores and gate loads: lane q of the four takes the q-th 16 bytes of 64 of each row.
+      const long long row = x.c0 + i_tok;
+      const bool gated = a.gate && a.splits == 1;
+      long long o_off[4], g_off[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int src = (lane & ~3) + j;
+        const long long rj = __shfl_sync(0xFFFFFFFFu, valid ? row : -1, src);
+        const int hj = __shfl_sync(0xFFFFFFFFu, h, src);
+        o_off[j] = rj < 0 ? -1 : (rj * a.nq + hj) * Dh + 8 * (lane & 3);
+        g_off[j] = rj * a.gate_ld + hj * a.gate_hs + 8 * (lane & 3);
+      }
+      constexpr int AHEAD = 2;  // chunks of 32 dims whose gates are fetched ahead
+      uint4 gates[AHEAD][4];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (gated && o_off[j] >= 0) gates[k][j] = *reinterpret_cast<const uint4*>(a.gate + g_off[j] + 32 * k);
+      g += ts.subs;
       if (nt > 0) {
-        bar_wait(&bars->dead, &bars->done[w], 0, a.err);
+        pvs += ts.subs - 1;
+        warp_wait(&bars->dead, &bars->done[w], finished & 1, a.err);
+        ++finished;
         tc_fence_after();
       }
       // O / l, gate, store; a row with an infinity or NaN is settled by the definition afterwards
-      const long long row = c0 + i_tok;
       const long long orow = (row * a.nq + h) * Dh;
       const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-      float* part = a.ws_o + (long long)split * a.T * a.nq * Dh + orow;
-      bool odd = false;
-#pragma unroll 1
+      float* part = a.ws_o + (long long)x.split * a.T * a.nq * Dh + orow;
+      float probe[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // 0 unless O holds an infinity or NaN
+#pragma unroll
       for (int d = 0; d < Dh; d += 32) {
         float o[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = gates[d / 32 % AHEAD][j];
+          if (gated && d + 32 * AHEAD < Dh && o_off[j] >= 0)
+            gates[d / 32 % AHEAD][j] = *reinterpret_cast<const uint4*>(a.gate + g_off[j] + d + 32 * AHEAD);
+        }
         if (nt > 0) {
           tmem_ld32_nowait(t_o + d, o);
           tmem_ld32_ready(o);
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) odd |= !isfinite(o[i]);
-        if (valid && a.splits > 1) {
+        for (int i = 0; i < 32; ++i) probe[i & 3] = __fmaf_rn(o[i], 0.0f, probe[i & 3]);
+        if (a.splits > 1) {
+          if (valid)
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(part + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else if (valid) {
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(part + d + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = __fmul_rn(o[i], inv);
-          if (a.gate) {
+          if (gated) {
+            transpose4(v, lane);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint4 g4 = *reinterpret_cast<const uint4*>(a.gate + row * a.gate_ld + h * a.gate_hs + d + 8 * i);
-              const uint32_t u[4] = {g4.x, g4.y, g4.z, g4.w};
+              const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                o[8 * i + 2 * x] = __fdividef(o[8 * i + 2 * x], 1.0f + ex2(-kLog2e * bflo(u[x])));
-                o[8 * i + 2 * x + 1] = __fdividef(o[8 * i + 2 * x + 1], 1.0f + ex2(-kLog2e * bfhi(u[x])));
+              for (int k = 0; k < 4; ++k) {
+                o[8 * i + 2 * k] = __fmul_rn(o[8 * i + 2 * k], sigmoid_fast(bflo(u[k])));
+                o[8 * i + 2 * k + 1] = __fmul_rn(o[8 * i + 2 * k + 1], sigmoid_fast(bfhi(u[k])));
               }
             }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(a.out + orow + d + 8 * i) =
-                make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]), pack_bf16(o[8 * i + 2], o[8 * i + 3]),
-                           pack_bf16(o[8 * i + 4], o[8 * i + 5]), pack_bf16(o[8 * i + 6], o[8 * i + 7]));
+            v[i] = make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]), pack_bf16(o[8 * i + 2], o[8 * i + 3]),
+                              pack_bf16(o[8 * i + 4], o[8 * i + 5]), pack_bf16(o[8 * i + 6], o[8 * i + 7]));
+          transpose4(v, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (o_off[j] >= 0) *reinterpret_cast<uint4*>(a.out + o_off[j] + d) = v[j];
         }
         __syncwarp();
       }
-      if (valid && a.splits > 1) a.ws_ml[((long long)split * a.T + row) * a.nq + h] = make_float2(m, l);
+      const bool odd = !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
+      tc_fence_before();
+      if (valid && a.splits > 1) a.ws_ml[((long long)x.split * a.T + row) * a.nq + h] = make_float2(m, l);
       unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && valid);
       while (todo) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
-        const int rr = (tid & 127 & ~31) + src, ti = tok0 + w * a.tpt + rr / a.G, hh = kh * a.G + rr % a.G;
-        const long long tr = c0 + ti;
+        const int rr = (tid & 127 & ~31) + src, ti = x.tok0 + w * a.tpt + rr / a.G, hh = x.kh * a.G + rr % a.G;
+        const long long tr = x.c0 + ti;
         float mm = -INFINITY, ll = 0.0f, oo[Dh / 32] = {};
         for (int t = 0; t < nt; ++t)
-          attend_row_strict<Dh>(c, a.q + tr * a.q_ld + (long long)hh * Dh, b, kh, len - n + ti, tile_key(t),
-                                tile_key(t) + kKeys, a.vis, a.scale2, a.err, mm, ll, oo);
+          attend_row_strict<Dh>(c, a.q + tr * a.q_ld + (long long)hh * Dh, x.b, x.kh, x.len - x.n + ti, ts.key(t),
+                                ts.key(t) + kKeys, a.vis, a.scale2, a.err, mm, ll, oo);
         __syncwarp();
         for (int e = 0; e < Dh / 32; ++e) {
           const int d = lane * (Dh / 32) + e;
           const long long at = (tr * a.nq + hh) * Dh + d;
           if (a.splits > 1) {
-            a.ws_o[(long long)split * a.T * a.nq * Dh + at] = oo[e];
+            a.ws_o[(long long)x.split * a.T * a.nq * Dh + at] = oo[e];
           } else {
             float y = __fdiv_rn(oo[e], ll);
             if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[tr * a.gate_ld + hh * a.gate_hs + d])));
             a.out[at] = f2bf(y);
           }
         }
-        if (a.splits > 1 && lane == 0) a.ws_ml[((long long)split * a.T + tr) * a.nq + hh] = make_float2(mm, ll);
+        if (a.splits > 1 && lane == 0) a.ws_ml[((long long)x.split * a.T + tr) * a.nq + hh] = make_float2(mm, ll);
       }
     }
   }
@@ -566,18 +719,19 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedView c, PromptArg
 }
 
 // ----------------------------------------------------------------------------- host
-// CTAs that a call needs at most (the sequences' row counts are only known on the device).
+// Items of work that a call has at most (the sequences' row counts are only known on the device).
 static long long prompt_items(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
   const int NQ = c->Dh == 256 ? 1 : 2, TT = NQ * (kRows / (a->n_q / c->n_kv));
   return ((long long)a->T / TT + std::min(a->T, c->B)) * c->n_kv;
 }
 
-// With fewer CTAs than SMs the key tiles of each are split, down to two tiles a split.
+// With fewer items than SMs the key tiles of each are split, down to four tiles a split: two (512 tokens of 16 / 4
+// heads of 256 in 128 CTAs) measured 25.1 us, whole items (64 CTAs) 18.1; 128 tokens behind 8000 want the split, 38 for 117 us.
 static int prompt_splits(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
   const long long items = prompt_items(a, c), sms = sm_count();
   long long tiles = ((long long)c->table_w * c->page + kKeys - 1) / kKeys;
   if (a->window > 0) tiles = std::min(tiles, ((long long)a->window + kRows) / kKeys + 2 + a->sinks / kKeys);
-  return int(std::max<long long>(1, std::min({sms / items, tiles / 2, 32ll})));
+  return int(std::max<long long>(1, std::min({sms / items, tiles / 4, 32ll})));
 }
 
 template <int Dh>
@@ -596,8 +750,7 @@ static int launch_prompt(const qmtp_paged_args* args, const PagedView& v, const 
   const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kKeys / Cfg::E))};
   if (!encode_pages(&tq, a.q, 3, qd, qs, qb) || !encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb))
     return QMTP_ERR_CUDA;
-  launch_kernel(paged_prompt_kernel<Dh>, dim3(unsigned(items), unsigned(a.splits)), dim3(Cfg::threads), Cfg::smem, st, tq, tk,
-                tv, v, a);
+  launch_kernel(paged_prompt_kernel<Dh>, dim3(unsigned(items * a.splits)), dim3(Cfg::threads), Cfg::smem, st, tq, tk, tv, v, a);
   if (a.splits > 1)
     launch_kernel(prompt_join_kernel<Dh>, dim3(unsigned(((long long)a.T * a.nq + 7) / 8)), dim3(256), 0, st, v, a);
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
