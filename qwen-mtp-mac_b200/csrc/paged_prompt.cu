@@ -598,7 +598,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
       float* part = a.ws_o + (long long)x.split * a.T * a.nq * Dh + orow;
       float probe[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // 0 unless O holds an infinity or NaN
-#pragma unroll
+#pragma unroll 2  // not more: code that runs once an item costs instruction fetches (8 chunks unrolled: +2 us)
       for (int d = 0; d < Dh; d += 32) {
         float o[32];
 #pragma unroll
