@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <cmath>
 
+#include <cuda_bf16.h>
+
 #include "paged.cuh"
 
 namespace qmtp {
@@ -163,6 +165,8 @@ struct DecodeArgs {
   float* ws_o;    // [B][max_slabs][S * nq][Dh] numerators
   float2* ws_ml;  // [B][max_slabs][S * nq] running maximum (base 2) and sum
   int nq, S, G, row_tiles, max_slabs, fine;
+  int one_round;   // no CTA has a second unit
+  unsigned inv_g;  // ceil(2^16 / G): r / G = r * inv_g >> 16 for r < 512, G <= 64
   float scale2;   // scale * log2(e)
   Visible vis;
   unsigned* err;
@@ -213,7 +217,7 @@ struct DecodeSmem {
   uint16_t kv[DecodeCfg<Dh>::ring][kTile * Dh];  // 64-dim column blocks of 128-byte swizzled rows
   static constexpr int QS = NT == 2 ? 1 : 2;  // per_sm CTAs have to fit on an SM
   uint16_t q[QS][8 * NT][Dh + 8];
-  uint16_t p[8 * NT][kTile + 8];  // weights, [row][key]
+  __nv_bfloat16 p[8 * NT][kTile + 8];  // weights, [row][key]
   float mx[4][8 * NT];
   float sum[2][4][8 * NT];
   uint64_t full[DecodeCfg<Dh>::ring], empty[DecodeCfg<Dh>::ring], q_full[2], q_empty[2];
@@ -224,14 +228,35 @@ struct DecodeSmem {
 
 struct DecodeUnit {
   int b, kh, row0, len, lo, k_begin, k_end, part;
-  bool whole;
 };
+
+// Unit u of the call: s_pre the slabs before every sequence, s_len their lengths.  Not inlined: the producer and the
+// consumers call it once a unit, and the kernel's code is fetched anew for every launch.
+__device__ __noinline__ DecodeUnit decode_unit(const int* s_pre, const int* s_len, const DecodeArgs& a, int B, int nkv,
+                                               int rows, int u) {
+  DecodeUnit x;
+  const int per = nkv * a.row_tiles, slab_g = u / per, rest = u - slab_g * per;
+  x.kh = rest / a.row_tiles;
+  x.row0 = (rest - x.kh * a.row_tiles) * rows;
+  int b = 0;  // the last sequence that begins at or before this slab
+  for (int step = 1 << (31 - __clz(B)); step > 0; step >>= 1)
+    if (b + step < B && s_pre[b + step] <= slab_g) b += step;
+  x.b = b;
+  x.len = s_len[b];
+  const SlabList sl = slab_list(a, x.len);
+  x.lo = sl.lo;
+  x.part = slab_g - s_pre[b];
+  const int slab = x.part < sl.first ? x.part : sl.from + x.part - sl.first;
+  x.k_begin = slab_begin(slab, a.fine);
+  x.k_end = min(slab_begin(slab + 1, a.fine), x.len);
+  return x;
+}
 
 template <int Dh, int NT>
 __global__ void __launch_bounds__(160, DecodeCfg<Dh>::per_sm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, PagedView c,
-                    DecodeArgs a) {
-  pdl_trigger();
+                    const __grid_constant__ DecodeArgs a) {
+  if (a.one_round) pdl_trigger();  // otherwise when the last unit is done: a waiting successor's blocks take up room
   extern __shared__ uint8_t smem_raw[];
   using Smem = DecodeSmem<Dh, NT>;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -264,25 +289,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
   if (tid == 0) s_pre[c.B] = total;
   __syncthreads();
   const int R = a.S * a.G, per = c.nkv * a.row_tiles, units = total * per;
-  auto unit_at = [&](int u) {
-    DecodeUnit x;
-    const int slab_g = u / per, rest = u - slab_g * per;
-    x.kh = rest / a.row_tiles;
-    x.row0 = (rest - x.kh * a.row_tiles) * 8 * NT;
-    int b = 0;  // the last sequence that begins at or before this slab
-    for (int step = 1 << (31 - __clz(c.B)); step > 0; step >>= 1)
-      if (b + step < c.B && s_pre[b + step] <= slab_g) b += step;
-    x.b = b;
-    x.len = s_len[b];
-    const SlabList sl = slab_list(a, x.len);
-    x.lo = sl.lo;
-    x.part = slab_g - s_pre[b];
-    const int slab = x.part < sl.first ? x.part : sl.from + x.part - sl.first;
-    x.k_begin = slab_begin(slab, a.fine);
-    x.k_end = min(slab_begin(slab + 1, a.fine), x.len);
-    x.whole = sl.count == 1;  // the only slab: its result is final
-    return x;
-  };
+  auto unit_at = [&](int u) { return decode_unit(s_pre, s_len, a, c.B, c.nkv, 8 * NT, u); };
   // the next tile of the unit, from key j on, that holds a needed key
   auto next_tile = [&](const DecodeUnit& x, int j) {
     while (j < x.k_end && a.vis.window != 0 && j + kTile <= x.lo && j >= a.vis.sinks) j += kTile;
@@ -344,7 +351,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         if (lane == 0) mbar_expect_tx(&sm.q_full[st], rows * Dh * 2);
         __syncwarp();
         if (lane < rows) {
-          const int r = x.row0 + lane, s = r / a.G;
+          const int r = x.row0 + lane, s = r * a.inv_g >> 16;
           bulk_g2s(sm.q[st][lane], a.q + (long long)(x.b * a.S + s) * a.q_ld + (long long)(x.kh * a.G + r - s * a.G) * Dh,
                    Dh * 2, &sm.q_full[st], policy_evict_last());
         }
@@ -376,7 +383,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = x.row0 + 8 * t + 2 * quad + i;
-        prow[t][i] = r < R ? pos0 + r / a.G : -1;
+        prow[t][i] = r < R ? pos0 + int(r * a.inv_g >> 16) : -1;
         m[t][i] = kNone;
         l[t][i] = 0.0f;
       }
@@ -448,8 +455,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
           l[t][i] = __fmaf_rn(l[t][i], alpha[t][i], __fadd_rn(p0, p1));
           // the weights enter the second product as bf16 (relative error 2^-9 each, against the
           // output's own bf16 rounding of the same size); their sum l keeps all 32 bits
-          sm.p[n][16 * warp + oct] = f2bf(p0);
-          sm.p[n][16 * warp + oct + 8] = f2bf(p1);
+          sm.p[n][16 * warp + oct] = __float2bfloat16_rn(p0);
+          sm.p[n][16 * warp + oct + 8] = __float2bfloat16_rn(p1);
         }
       warp_wait(&sm.dead, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
       if (j + kTile > x.len || (a.vis.window != 0 && j < x.lo)) {
@@ -494,6 +501,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.q_empty[uq % QS]);
+    if (u + int(gridDim.x) >= units) pdl_trigger();
     // sums over the key lanes and warps; is the numerator finite?
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -511,118 +519,189 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     consumers_sync();
     const bool odd = sm.bad[set] != 0;
     if (tid == 0) sm.bad[set ^ 1] = 0;
-    const long long part = (long long)x.b * a.max_slabs + x.part;
-    auto store = [&](int r, int d, float val, float ll) {
-      const int s = r / a.G, h = x.kh * a.G + r - s * a.G;
-      if (x.whole) {
-        const long long t = x.b * a.S + s;
-        float y = ll == 0.0f ? 0.0f : __fdiv_rn(val, ll);
-        if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[t * a.gate_ld + h * a.gate_hs + d])));
-        a.out[(t * a.nq + h) * Dh + d] = f2bf(y);
-      } else {
-        a.ws_o[((part * a.S + s) * a.nq + h) * Dh + d] = val;
-      }
-    };
+    const long long part = ((long long)x.b * a.max_slabs + x.part) * a.S;
     if (!odd) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int n = 8 * t + 2 * quad + i, r = x.row0 + n;
+          const int n = 8 * t + 2 * quad + i, r = x.row0 + n, s = r * a.inv_g >> 16;
           if (r >= R) continue;
-          const float ll = __fadd_rn(__fadd_rn(sm.sum[set][0][n], sm.sum[set][1][n]),
-                                     __fadd_rn(sm.sum[set][2][n], sm.sum[set][3][n]));
+          const long long at = (part + s) * a.nq + x.kh * a.G + r - s * a.G;
+          float* dst = a.ws_o + at * Dh + warp * MT * 16 + oct;
 #pragma unroll
           for (int y = 0; y < MT; ++y) {
-            const int d = (warp * MT + y) * 16 + oct;
-            store(r, d, o[y][t][i], ll);
-            store(r, d + 8, o[y][t][i + 2], ll);
+            dst[16 * y] = o[y][t][i];
+            dst[16 * y + 8] = o[y][t][i + 2];
           }
-          if (!x.whole && warp == 0 && oct == 0) {
-            const int s = r / a.G;
-            a.ws_ml[(part * a.S + s) * a.nq + x.kh * a.G + r - s * a.G] = make_float2(m[t][i], ll);
-          }
+          if (warp == 0 && oct == 0)
+            a.ws_ml[at] = make_float2(m[t][i], __fadd_rn(__fadd_rn(sm.sum[set][0][n], sm.sum[set][1][n]),
+                                                         __fadd_rn(sm.sum[set][2][n], sm.sum[set][3][n])));
         }
       __syncwarp();
     } else {
       // An infinity or NaN reached a sum: from a key that the row sees, or, as 0 * inf, from one it does not.
       // Settle it by the definition, a warp per row, reading visible keys only.
       for (int n = warp; n < 8 * NT && x.row0 + n < R; n += 4) {
-        const int r = x.row0 + n, s = r / a.G, h = x.kh * a.G + r - s * a.G;
+        const int r = x.row0 + n, s = r * a.inv_g >> 16, h = x.kh * a.G + r - s * a.G;
         float mm = kNone, ll = 0.0f, oo[Dh / 32] = {};
         attend_row_strict<Dh>(c, a.q + (long long)(x.b * a.S + s) * a.q_ld + (long long)h * Dh, x.b, x.kh, pos0 + s,
                               x.k_begin, x.k_end, a.vis, a.scale2, a.err, mm, ll, oo);
-        for (int i = 0; i < Dh / 32; ++i) store(r, lane * (Dh / 32) + i, oo[i], ll);
-        if (!x.whole && lane == 0) a.ws_ml[(part * a.S + s) * a.nq + h] = make_float2(mm, ll);
+        const long long at = (part + s) * a.nq + h;
+        for (int i = 0; i < Dh / 32; ++i) a.ws_o[at * Dh + lane * (Dh / 32) + i] = oo[i];
+        if (lane == 0) a.ws_ml[at] = make_float2(mm, ll);
       }
     }
   }
 }
 
-// Joins a row's slabs: M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.  A slab's class is its number mod
-// 16; every class is summed in order with its own running maximum, then the classes in order, so the
-// order of additions belongs to the slabs' positions, however the classes are dealt to threads.  A block takes
-// `4 * QB` dims of a row: QB lanes of 4 dims, 256 / QB groups of QB / 16 classes each.  QB = 16 when rows are few
-// (every class its own threads), Dh / 4 when there are enough rows to fill the GPU.
-template <int Dh, int QB>
-__global__ void __launch_bounds__(256) paged_join_kernel(PagedView c, DecodeArgs a) {
+// Joins a row's slabs: M = max m_i, o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i, the gate, the rounding.  A slab's class
+// is its number mod 16; every class is summed in rising order, then the classes in order, so the order of
+// additions belongs to the slabs' positions, however they are dealt to threads.  Two ways to deal them:
+//   wide (few rows): a block per (row, 64 dims), 16 threads of 4 dims for each class;
+//   warp (many rows): a warp per (row, 128 dims), 4 dims a lane and every class in its registers, no barrier.
+struct JoinRow {
+  const float2* ml;   // slab i at ml[i * stride]
+  const float* o;     // ... at o[i * stride * Dh]
+  long long out, gate, stride;
+  SlabList sl;
+};
+template <int Dh>
+__device__ __forceinline__ JoinRow join_row(const PagedView& c, const DecodeArgs& a, int br) {
+  JoinRow j;
+  const int rows = a.S * a.nq, b = br / rows, r = br - b * rows, s = r / a.nq, h = r - s * a.nq;
+  j.sl = slab_list(a, seq_len(c, b, nullptr));
+  j.ml = a.ws_ml + (long long)b * a.max_slabs * rows + r;
+  j.o = a.ws_o + ((long long)b * a.max_slabs * rows + r) * Dh;
+  j.stride = rows;
+  const long long t = b * a.S + s;
+  j.out = (t * a.nq + h) * Dh;
+  j.gate = t * a.gate_ld + h * a.gate_hs;
+  return j;
+}
+__device__ __forceinline__ float join_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M)); }
+
+template <int Dh>
+__global__ void __launch_bounds__(256) paged_join_wide_kernel(PagedView c, DecodeArgs a) {
   pdl_trigger();
   pdl_wait();
-  constexpr int CPT = QB / 16, BPR = Dh / (4 * QB);  // classes per thread, blocks per row
-  __shared__ float4 s_o[16][QB];
-  __shared__ float2 s_ml[16];
-  const int tid = threadIdx.x, g = tid / QB, ln = tid - g * QB;
-  const int br = blockIdx.x / BPR, d0 = (blockIdx.x - br * BPR) * 4 * QB;
-  const int rows = a.S * a.nq, b = br / rows, r = br - b * rows;  // r = s * nq + h
-  const SlabList sl = slab_list(a, seq_len(c, b, nullptr));
-  if (sl.count == 1) return;
-  const float2* ml = a.ws_ml + (long long)b * a.max_slabs * rows + r;
-  const float* po = a.ws_o + ((long long)b * a.max_slabs * rows + r) * Dh + d0 + 4 * ln;
+  __shared__ float s_m[8];
+  __shared__ float4 s_o[16][16];
+  __shared__ float s_l[16];
+  const int tid = threadIdx.x, lane = tid & 31, cls = tid >> 4, d0 = blockIdx.x % (Dh / 64) * 64;
+  const JoinRow j = join_row<Dh>(c, a, blockIdx.x / (Dh / 64));
+  float gate = 0.0f;
+  if (a.gate && tid < 64) gate = bf2f(a.gate[j.gate + d0 + tid]);
+  float M = -INFINITY;
+  for (int i = tid; i < j.sl.count; i += 256) M = fmaxf(M, j.ml[i * j.stride].x);
 #pragma unroll
-  for (int k = 0; k < CPT; ++k) {
-    const int cls = g * CPT + k;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float M = -INFINITY, den = 0.0f;
-    // listed slab i has number i (i < first) or from + i - first: a class begins at its residue
-    auto walk = [&](int i0, int i1, int number0) {
-#pragma unroll 4
-      for (int i = i0 + ((cls - number0) & 15); i < i1; i += 16) {
-        const float2 v = ml[(long long)i * rows];
-        const float4 x = *reinterpret_cast<const float4*>(po + (long long)i * rows * Dh);
-        if (v.x == -INFINITY && v.y == 0.0f) continue;  // a slab this row sees nothing of
-        const float mn = fmaxf(M, v.x), safe = mn == -INFINITY ? 0.0f : mn;
-        const float w = ex2(__fsub_rn(v.x, safe)), f = ex2(__fsub_rn(M, safe));
-        M = mn;
-        den = __fmaf_rn(den, f, __fmul_rn(w, v.y));
-        acc.x = __fmaf_rn(acc.x, f, __fmul_rn(w, x.x));
-        acc.y = __fmaf_rn(acc.y, f, __fmul_rn(w, x.y));
-        acc.z = __fmaf_rn(acc.z, f, __fmul_rn(w, x.z));
-        acc.w = __fmaf_rn(acc.w, f, __fmul_rn(w, x.w));
-      }
-    };
-    walk(0, sl.first, 0);
-    walk(sl.first, sl.count, sl.from);
-    s_o[cls][ln] = acc;
-    if (ln == 0) s_ml[cls] = make_float2(M, den);
-  }
+  for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, x));
+  if (lane == 0) s_m[tid >> 5] = M;
   __syncthreads();
-  if (tid >= 4 * QB) return;
-  float M = -INFINITY, y = 0.0f, ll = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) M = fmaxf(M, s_ml[i].x);
-  const float safe = M == -INFINITY ? 0.0f : M;
+  for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.0f;
+  const float* po = j.o + d0 + 4 * (tid & 15);
+  // listed slab i has number i (i < first) or from + i - first: a class begins at its residue
+  for (int part = 0; part < 2; ++part) {
+    const int i0 = part ? j.sl.first : 0, i1 = part ? j.sl.count : j.sl.first, number0 = part ? j.sl.from : 0;
+#pragma unroll 16
+    for (int i = i0 + ((cls - number0) & 15); i < i1; i += 16) {
+      const float2 v = j.ml[i * j.stride];
+      const float4 x = *reinterpret_cast<const float4*>(po + i * j.stride * Dh);
+      const float w = join_weight(v.x, M);
+      den = __fmaf_rn(w, v.y, den);
+      acc.x = __fmaf_rn(w, x.x, acc.x);
+      acc.y = __fmaf_rn(w, x.y, acc.y);
+      acc.z = __fmaf_rn(w, x.z, acc.z);
+      acc.w = __fmaf_rn(w, x.w, acc.w);
+    }
+  }
+  s_o[cls][tid & 15] = acc;
+  if ((tid & 15) == 0) s_l[cls] = den;
+  __syncthreads();
+  if (tid >= 64) return;
   const float* so = reinterpret_cast<const float*>(s_o);
+  float y = 0.0f, ll = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float f = ex2(__fsub_rn(s_ml[i].x, safe));
-    y = __fmaf_rn(f, so[i * 4 * QB + tid], y);
-    ll = __fmaf_rn(f, s_ml[i].y, ll);
+    y = __fadd_rn(y, so[i * 64 + tid]);
+    ll = __fadd_rn(ll, s_l[i]);
   }
   y = ll == 0.0f ? 0.0f : __fdiv_rn(y, ll);
-  const int s = r / a.nq, h = r - s * a.nq, d = d0 + tid;
-  const long long t = b * a.S + s;
-  if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[t * a.gate_ld + h * a.gate_hs + d])));
-  a.out[(t * a.nq + h) * Dh + d] = f2bf(y);
+  if (a.gate) y = __fmul_rn(y, sigmoid_f32(gate));
+  a.out[j.out + d0 + tid] = f2bf(y);
+}
+
+template <int Dh>
+__global__ void __launch_bounds__(128) paged_join_warp_kernel(PagedView c, DecodeArgs a) {
+  pdl_wait();
+  constexpr int LPR = Dh / 4, RPW = LPR < 32 ? 32 / LPR : 1, WPR = LPR > 32 ? LPR / 32 : 1;  // lanes a row, rows a warp
+  const int lane = threadIdx.x & 31, wid = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int br = wid / WPR * RPW + (RPW > 1 ? lane / LPR : 0), d = RPW > 1 ? lane % LPR * 4 : (wid % WPR * 32 + lane) * 4;
+  const bool live = br < c.B * a.S * a.nq;
+  const JoinRow j = join_row<Dh>(c, a, live ? br : 0);
+  uint2 g2 = make_uint2(0, 0);
+  if (a.gate) g2 = *reinterpret_cast<const uint2*>(a.gate + j.gate + d);
+  // half-warp lane k looks after class k: its slabs' weights and its share of the denominator
+  const int k0 = lane & 15, half = lane & 16;
+  float M = -INFINITY, den = 0.0f;
+  for (int i = k0; i < j.sl.count; i += 16) M = fmaxf(M, j.ml[i * j.stride].x);
+#pragma unroll
+  for (int x = 8; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, x));
+  const long long step = j.stride * Dh;
+  float4 acc[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    // slabs i0 .. i1 of the list have numbers number0 ..: sixteen numbers, one of each class, at a time
+    const int i0 = part ? j.sl.first : 0, i1 = part ? j.sl.count : j.sl.first, number0 = part ? j.sl.from : 0;
+#pragma unroll 1
+    for (int i = i0 - (number0 & 15); __any_sync(0xFFFFFFFFu, i < i1); i += 16) {
+      float w = 0.0f;
+      if (i + k0 >= i0 && i + k0 < i1) {
+        const float2 v = j.ml[(i + k0) * j.stride];
+        w = join_weight(v.x, M);
+        den = __fmaf_rn(w, v.y, den);
+      }
+      const float* po = j.o + d;
+#pragma unroll
+      for (int h = 0; h < 16; h += 8) {
+        float4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)  // eight loads under way at once; a number outside the list has weight 0
+          x[k] = *reinterpret_cast<const float4*>(po + min(max(i + h + k, 0), j.sl.count - 1) * step);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float wk = __shfl_sync(0xFFFFFFFFu, w, half + h + k);
+          acc[h + k].x = __fmaf_rn(wk, x[k].x, acc[h + k].x);
+          acc[h + k].y = __fmaf_rn(wk, x[k].y, acc[h + k].y);
+          acc[h + k].z = __fmaf_rn(wk, x[k].z, acc[h + k].z);
+          acc[h + k].w = __fmaf_rn(wk, x[k].w, acc[h + k].w);
+        }
+      }
+    }
+  }
+  float y[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    y[0] = __fadd_rn(y[0], acc[k].x);
+    y[1] = __fadd_rn(y[1], acc[k].y);
+    y[2] = __fadd_rn(y[2], acc[k].z);
+    y[3] = __fadd_rn(y[3], acc[k].w);
+    ll = __fadd_rn(ll, __shfl_sync(0xFFFFFFFFu, den, half + k));
+  }
+  const float g[4] = {bflo(g2.x), bfhi(g2.x), bflo(g2.y), bfhi(g2.y)};
+  uint16_t h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    y[k] = ll == 0.0f ? 0.0f : __fdiv_rn(y[k], ll);
+    if (a.gate) y[k] = __fmul_rn(y[k], sigmoid_f32(g[k]));
+    h[k] = f2bf(y[k]);
+  }
+  if (live) *reinterpret_cast<uint2*>(a.out + j.out + d) = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -669,7 +748,7 @@ static int max_slabs(const qmtp_paged_args* a, const qmtp_paged_cache* c, int S)
 static size_t align_up(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <int Dh, int NT>
-static int launch_decode(const PagedView& v, const DecodeArgs& a, long long units, cudaStream_t st) {
+static int launch_decode(const PagedView& v, DecodeArgs a, long long units, cudaStream_t st) {
   constexpr size_t fixed = sizeof(DecodeSmem<Dh, NT>) + 1024;
   static DeviceOnce ready;
   if (!ready([] {
@@ -682,13 +761,14 @@ static int launch_decode(const PagedView& v, const DecodeArgs& a, long long unit
   const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kTile))};
   if (!encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb)) return QMTP_ERR_CUDA;
   const int grid = int(std::min<long long>(units, (long long)sm_count() * DecodeCfg<Dh>::per_sm));
+  a.one_round = grid == units;
   launch_kernel(paged_decode_kernel<Dh, NT>, dim3(grid), dim3(160), fixed + (2 * v.B + 1) * sizeof(int), st, tk, tv, v, a);
-  if (a.max_slabs > 1) {
-    const int rows = v.B * a.S * a.nq;
-    if (rows >= 2 * sm_count())
-      launch_kernel(paged_join_kernel<Dh, Dh / 4>, dim3(rows), dim3(256), 0, st, v, a);
-    else
-      launch_kernel(paged_join_kernel<Dh, 16>, dim3(rows * (Dh / 64)), dim3(256), 0, st, v, a);
+  const int rows = v.B * a.S * a.nq;
+  if (rows >= 2 * sm_count()) {
+    constexpr int RPW = Dh == 64 ? 2 : 1, WPR = Dh == 256 ? 2 : 1;
+    launch_kernel(paged_join_warp_kernel<Dh>, dim3((((rows + RPW - 1) / RPW) * WPR + 3) / 4), dim3(128), 0, st, v, a);
+  } else {
+    launch_kernel(paged_join_wide_kernel<Dh>, dim3(rows * (Dh / 64)), dim3(256), 0, st, v, a);
   }
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
 }
@@ -730,9 +810,9 @@ extern "C" int qmtp_paged_append(const void* qkv, long long ld, int T, const int
 }
 
 extern "C" size_t qmtp_paged_attention_workspace(const qmtp_paged_args* args, const qmtp_paged_cache* cache) {
-  if (!args || !cache || cache->B < 1 || cache->table_w < 1 || cache->page < 1) return 0;
+  PagedView v;
+  if (paged_view(cache, &v) || paged_check_args(args, cache)) return 0;
   const int S = args->T / cache->B, n = max_slabs(args, cache, S);
-  if (n <= 1) return 0;
   const size_t rows = size_t(cache->B) * n * S * args->n_q;
   return align_up(rows * cache->Dh * sizeof(float)) + rows * sizeof(float2);
 }
@@ -746,9 +826,9 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   const int S = args->T / v.B, G = args->n_q / v.nkv;
   if (S > kMaxS) return QMTP_ERR_UNSUPPORTED;
   const size_t need = qmtp_paged_attention_workspace(args, cache);
-  if (need && !workspace) return QMTP_ERR_ARG;
+  if (!workspace) return QMTP_ERR_ARG;
   if (ws_bytes < need) return QMTP_ERR_SHAPE;
-  if (need && !aligned16(workspace)) return QMTP_ERR_ALIGN;
+  if (!aligned16(workspace)) return QMTP_ERR_ALIGN;
   unsigned* err = device_error_ptr();
   if (!err) return QMTP_ERR_CUDA;
   DecodeArgs a{};
@@ -761,6 +841,7 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   a.nq = args->n_q;
   a.S = S;
   a.G = G;
+  a.inv_g = (65536 + G - 1) / G;
   a.scale2 = args->scale * kLog2e;
   a.vis = Visible{args->window, args->sinks};
   a.fine = fine_slabs(args->window);

@@ -72,7 +72,7 @@ def test_attention_workspace():
     long = cache(table_w=100, ld_table=100)
     n = L.qmtp_paged_attention_workspace(ctypes.byref(attn()), ctypes.byref(long))
     assert n >= 2 * 13 * 2 * 4 * (128 + 2) * 4  # B x slabs of 128 in 1600 x S x heads x (head_dim + 2) floats
-    assert L.qmtp_paged_attention_workspace(ctypes.byref(attn()), ctypes.byref(cache())) == 0  # 64 tokens: one slab
+    assert L.qmtp_paged_attention_workspace(ctypes.byref(attn()), ctypes.byref(cache(B=0))) == 0  # a refused call
     call = lambda ws, size: L.qmtp_paged_attention(ctypes.byref(attn()), ctypes.byref(long), ws, size, None)
     assert call(None, n) == ARG and call(PTR, n - 1) == SHAPE and call(PTR + 8, n) == ALIGN
     # a window needs the slabs it can touch, not the whole table's
