@@ -141,7 +141,6 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
 // time the bytes take.  A CTA takes units u, u + grid, ...; its producer warp walks their tiles ahead of the four
 // consumer warps and keeps the ring full across units, so neither a unit's first load nor its table
 // lookups are waited for.
-constexpr int kTile = 64;      // keys per step: 16 a warp for the scores
 constexpr int kFineSlab = 128; // slab sizes: see slab_of
 constexpr int kFineKeys = 4096;
 constexpr int kSlab = 512;
@@ -206,21 +205,25 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 // Barrier of the four consumer warps.
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-template <int Dh>
+// NT: groups of 8 query rows in a tile (1, 2 or 4).  A step takes TK keys, 16 KG a warp for the scores; small heads take
+// more of them, which spreads a step's waits and barriers over more work.
+template <int Dh, int NT>
 struct DecodeCfg {
-  static constexpr int ring = Dh == 256 ? 3 : Dh == 128 ? 4 : 6;  // entries: a tile of K or of V each
-  static constexpr int per_sm = Dh == 256 ? 2 : Dh == 128 ? 3 : 4;
+  static constexpr int KG = Dh == 64 ? 2 : 1, TK = 64 * KG;
+  static constexpr int per_sm = Dh == 256 || NT == 4 ? 2 : 3;
+  static constexpr int ring = Dh == 256 ? 3 : NT < 4 ? 4 : 6;  // entries: a tile of K or of V each
 };
 
 template <int Dh, int NT>
 struct DecodeSmem {
-  uint16_t kv[DecodeCfg<Dh>::ring][kTile * Dh];  // 64-dim column blocks of 128-byte swizzled rows
-  static constexpr int QS = NT == 2 ? 1 : 2;  // per_sm CTAs have to fit on an SM
+  using Cfg = DecodeCfg<Dh, NT>;
+  uint16_t kv[Cfg::ring][Cfg::TK * Dh];  // 64-dim column blocks of 128-byte swizzled rows
+  static constexpr int QS = NT > 1 ? 1 : 2;  // per_sm CTAs have to fit on an SM
   uint16_t q[QS][8 * NT][Dh + 8];
-  __nv_bfloat16 p[8 * NT][kTile + 8];  // weights, [row][key]
+  __nv_bfloat16 p[8 * NT][Cfg::TK + 8];  // weights, [row][key]
   float mx[4][8 * NT];
   float sum[2][4][8 * NT];
-  uint64_t full[DecodeCfg<Dh>::ring], empty[DecodeCfg<Dh>::ring], q_full[2], q_empty[2];
+  uint64_t full[Cfg::ring], empty[Cfg::ring], q_full[2], q_empty[2];
   int bad[2];
   int scan[8];
   int dead;
@@ -253,7 +256,7 @@ __device__ __noinline__ DecodeUnit decode_unit(const int* s_pre, const int* s_le
 }
 
 template <int Dh, int NT>
-__global__ void __launch_bounds__(160, DecodeCfg<Dh>::per_sm)
+__global__ void __launch_bounds__(160, DecodeCfg<Dh, NT>::per_sm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, PagedView c,
                     const __grid_constant__ DecodeArgs a) {
   if (a.one_round) pdl_trigger();  // otherwise when the last unit is done: a waiting successor's blocks take up room
@@ -262,7 +265,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   int* s_pre = reinterpret_cast<int*>(&sm + 1);  // [B + 1] slabs before sequence b
   int* s_len = s_pre + c.B + 1;                  // [B]
-  constexpr int RING = DecodeCfg<Dh>::ring, CB = Dh / 64, QS = Smem::QS;
+  using Cfg = DecodeCfg<Dh, NT>;
+  constexpr int RING = Cfg::ring, CB = Dh / 64, QS = Smem::QS, KG = Cfg::KG, kTile = Cfg::TK;
   constexpr int MT = Dh / 64;  // 16-dim tiles of a warp in the weighted sum
   constexpr float kNone = -INFINITY;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -397,66 +401,85 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     for (int j = next_tile(x, x.k_begin); j < x.k_end; j = next_tile(x, j + kTile)) {
       const int sk = e % RING, sv = (e + 1) % RING;
       warp_wait(&sm.dead, &sm.full[sk], (e / RING) & 1, a.err);
-      float s[NT][4];
+      float s[KG][NT][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int g = 0; g < KG; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[g][t][i] = 0.0f;
       {
-        const int row = 16 * warp + (lane & 15);
+        const int row = 16 * KG * warp + (lane & 15);
         const uint32_t base = smem_u32(sm.kv[sk]) + row * 128;
 #pragma unroll
-        for (int k = 0; k < Dh / 32; ++k) {  // 32 dims: two K fragments, one load of query fragments per 8 rows
-          uint32_t k0[4], k1[4];
+        for (int k = 0; k < Dh / 32; ++k) {  // 32 dims: two K fragments a key group, one load of query fragments a row group
+          uint32_t k0[KG][4], k1[KG][4];
           const uint32_t cbase = base + (k >> 1) * kTile * 128;
           const int ch = (k & 1) * 4 + (lane >> 4);
-          ldsm_x4(k0, cbase + ((ch ^ (row & 7)) << 4));
-          ldsm_x4(k1, cbase + (((ch + 2) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int g = 0; g < KG; ++g) {
+            ldsm_x4(k0[g], cbase + g * 16 * 128 + ((ch ^ (row & 7)) << 4));
+            ldsm_x4(k1[g], cbase + g * 16 * 128 + (((ch + 2) ^ (row & 7)) << 4));
+          }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             uint32_t qf[4];
             ldsm_x4(qf, qbase + t * 8 * (Dh + 8) * 2 + k * 64);
-            mma_bf16(s[t], k0, qf[0], qf[1]);
-            mma_bf16(s[t], k1, qf[2], qf[3]);
+#pragma unroll
+            for (int g = 0; g < KG; ++g) {
+              mma_bf16(s[g][t], k0[g], qf[0], qf[1]);
+              mma_bf16(s[g][t], k1[g], qf[2], qf[3]);
+            }
           }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[sk]);
-      const bool all = j + kTile - 1 <= pos0 && (a.vis.window == 0 || j >= a.vis.first(x.len - 1));
+      if (j + kTile - 1 > pos0 || (a.vis.window != 0 && j < a.vis.first(x.len - 1))) {  // not every row sees every key
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+        for (int g = 0; g < KG; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = j + 16 * warp + oct + 8 * (i >> 1);
-          s[t][i] = all || a.vis(prow[t][i & 1], key) ? __fmul_rn(s[t][i], a.scale2) : kNone;
-        }
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!a.vis(prow[t][i & 1], j + 16 * KG * warp + 16 * g + oct + 8 * (i >> 1))) s[g][t][i] = kNone;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float v = fmaxf(s[t][i], s[t][i + 2]);
+          float v = fmaxf(s[0][t][i], s[0][t][i + 2]);
+#pragma unroll
+          for (int g = 1; g < KG; ++g) v = fmaxf(v, fmaxf(s[g][t][i], s[g][t][i + 2]));
 #pragma unroll
           for (int d = 4; d <= 16; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
           if (oct == 0) sm.mx[warp][8 * t + 2 * quad + i] = v;
         }
-      }
       consumers_sync();
       float alpha[NT][2];
+      bool grown = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int n = 8 * t + 2 * quad + i;
-          const float mn =
-              fmaxf(fmaxf(m[t][i], fmaxf(sm.mx[0][n], sm.mx[1][n])), fmaxf(sm.mx[2][n], sm.mx[3][n]));
-          const float safe = mn == kNone ? 0.0f : mn;  // nothing seen yet: every weight is 0
-          alpha[t][i] = ex2(__fsub_rn(m[t][i], safe));
+          const float top = fmaxf(fmaxf(sm.mx[0][n], sm.mx[1][n]), fmaxf(sm.mx[2][n], sm.mx[3][n]));
+          const float mn = fmaxf(m[t][i], __fmul_rn(top, a.scale2));
+          const float neg = mn == kNone ? 0.0f : -mn;  // nothing seen yet: every weight is 0
+          alpha[t][i] = ex2(__fadd_rn(m[t][i], neg));
+          grown |= mn != m[t][i];
           m[t][i] = mn;
-          const float p0 = ex2(__fsub_rn(s[t][i], safe)), p1 = ex2(__fsub_rn(s[t][i + 2], safe));
-          l[t][i] = __fmaf_rn(l[t][i], alpha[t][i], __fadd_rn(p0, p1));
-          // the weights enter the second product as bf16 (relative error 2^-9 each, against the
-          // output's own bf16 rounding of the same size); their sum l keeps all 32 bits
-          sm.p[n][16 * warp + oct] = __float2bfloat16_rn(p0);
-          sm.p[n][16 * warp + oct + 8] = __float2bfloat16_rn(p1);
+          float sum = 0.0f;
+#pragma unroll
+          for (int g = 0; g < KG; ++g) {
+            const float p0 = ex2(__fmaf_rn(s[g][t][i], a.scale2, neg)), p1 = ex2(__fmaf_rn(s[g][t][i + 2], a.scale2, neg));
+            sum = __fadd_rn(sum, __fadd_rn(p0, p1));
+            // the weights enter the second product as bf16 (relative error 2^-9 each, against the
+            // output's own bf16 rounding of the same size); their sum l keeps all 32 bits
+            sm.p[n][16 * KG * warp + 16 * g + oct] = __float2bfloat16_rn(p0);
+            sm.p[n][16 * KG * warp + 16 * g + oct + 8] = __float2bfloat16_rn(p1);
+          }
+          l[t][i] = __fmaf_rn(l[t][i], alpha[t][i], sum);
         }
       warp_wait(&sm.dead, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
       if (j + kTile > x.len || (a.vis.window != 0 && j < x.lo)) {
@@ -470,12 +493,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         fence_proxy_async();
       }
       consumers_sync();
+      if (__any_sync(0xFFFFFFFFu, grown)) {
 #pragma unroll
-      for (int y = 0; y < MT; ++y)
+        for (int y = 0; y < MT; ++y)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[y][t][i] = __fmul_rn(o[y][t][i], alpha[t][i & 1]);
+            for (int i = 0; i < 4; ++i) o[y][t][i] = __fmul_rn(o[y][t][i], alpha[t][i & 1]);
+      }
       const uint32_t vbase = smem_u32(sm.kv[sv]);
 #pragma unroll
       for (int k = 0; k < kTile / 16; ++k) {
@@ -758,9 +783,9 @@ static int launch_decode(const PagedView& v, DecodeArgs a, long long units, cuda
     return QMTP_ERR_CUDA;
   CUtensorMap tk, tv;
   const cuuint64_t kd[2] = {Dh, cuuint64_t((v.pages * v.nkv) << v.page_log)}, ks[1] = {Dh * 2};
-  const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kTile))};
+  const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, DecodeCfg<Dh, NT>::TK))};
   if (!encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb)) return QMTP_ERR_CUDA;
-  const int grid = int(std::min<long long>(units, (long long)sm_count() * DecodeCfg<Dh>::per_sm));
+  const int grid = int(std::min<long long>(units, (long long)sm_count() * DecodeCfg<Dh, NT>::per_sm));
   a.one_round = grid == units;
   launch_kernel(paged_decode_kernel<Dh, NT>, dim3(grid), dim3(160), fixed + (2 * v.B + 1) * sizeof(int), st, tk, tv, v, a);
   const int rows = v.B * a.S * a.nq;
@@ -850,12 +875,15 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) +
                                       align_up(size_t(v.B) * a.max_slabs * S * a.nq * cache->Dh * sizeof(float)));
-  const bool two = S * G > 8;
-  a.row_tiles = (S * G + (two ? 15 : 7)) / (two ? 16 : 8);
+  // rows of a tile: as many as there are up to 32, at 256 dims up to 16 (registers); K and V are read once a tile
+  const int nt = S * G <= 8 ? 1 : S * G <= 16 || cache->Dh == 256 ? 2 : 4;
+  a.row_tiles = (S * G + 8 * nt - 1) / (8 * nt);
   const long long units = (long long)v.B * a.max_slabs * v.nkv * a.row_tiles;
   if (units >= (1ll << 30) || (long long)v.B * S * a.nq >= (1ll << 28)) return QMTP_ERR_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define QMTP_DECODE(D) (two ? launch_decode<D, 2>(v, a, units, st) : launch_decode<D, 1>(v, a, units, st))
-  return cache->Dh == 64 ? QMTP_DECODE(64) : cache->Dh == 128 ? QMTP_DECODE(128) : QMTP_DECODE(256);
+#define QMTP_DECODE(D) (nt == 1 ? launch_decode<D, 1>(v, a, units, st) : launch_decode<D, 2>(v, a, units, st))
+  if (cache->Dh == 256) return QMTP_DECODE(256);
+  if (nt == 4) return cache->Dh == 64 ? launch_decode<64, 4>(v, a, units, st) : launch_decode<128, 4>(v, a, units, st);
+  return cache->Dh == 64 ? QMTP_DECODE(64) : QMTP_DECODE(128);
 #undef QMTP_DECODE
 }
