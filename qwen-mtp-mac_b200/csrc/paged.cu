@@ -141,21 +141,25 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
 // time the bytes take.  A CTA takes units u, u + grid, ...; its producer warp walks their tiles ahead of the four
 // consumer warps and keeps the ring full across units, so neither a unit's first load nor its table
 // lookups are waited for.
-constexpr int kFineSlab = 128; // slab sizes: see slab_of
 constexpr int kFineKeys = 4096;
-constexpr int kSlab = 512;
+constexpr int kSlabLog = 9;
 constexpr int kMaxS = 8;
 
-// Slabs have fixed positions: [0, 4096) in slabs of 128, then slabs of 512; 128 everywhere (fine) for windows up to
-// 4096.  Fine slabs spread a short context over the SMs (4 key heads x 2048 keys: 64 units); large ones keep the
-// partial results (Dh + 2 floats a row and slab) small next to the keys of a long one.  Fixed positions make a
-// row's arithmetic independent of the batch and of the call's other rows.
-__host__ __device__ inline int slab_of(int j, bool fine) {
-  return fine || j < kFineKeys ? j / kFineSlab : kFineKeys / kFineSlab + (j - kFineKeys) / kSlab;
-}
-__device__ __forceinline__ int slab_begin(int i, bool fine) {
-  return fine || i <= kFineKeys / kFineSlab ? i * kFineSlab : kFineKeys + (i - kFineKeys / kFineSlab) * kSlab;
-}
+// Slabs have fixed positions: [0, 4096) in fine slabs, then slabs of 512; fine ones everywhere for windows up to 4096.
+// Fine slabs spread a short context over the SMs: 128, 256 or 512 keys, so that the key heads of 4096 keys make
+// 128 units or more; larger ones keep the partial results (Dh + 2 floats a row and slab) small next to the keys.
+// Fixed positions make a row's arithmetic independent of the batch and of the call's other rows.
+struct Slabs {
+  int fine_log;
+  int all_fine;
+  __host__ __device__ __forceinline__ int of(int j) const {
+    return all_fine || j < kFineKeys ? j >> fine_log : (kFineKeys >> fine_log) + ((j - kFineKeys) >> kSlabLog);
+  }
+  __device__ __forceinline__ int begin(int i) const {
+    const int n = kFineKeys >> fine_log;
+    return all_fine || i <= n ? i << fine_log : kFineKeys + ((i - n) << kSlabLog);
+  }
+};
 
 struct DecodeArgs {
   const uint16_t *q, *gate;
@@ -163,7 +167,8 @@ struct DecodeArgs {
   long long q_ld, gate_ld, gate_hs;
   float* ws_o;    // [B][max_slabs][S * nq][Dh] numerators
   float2* ws_ml;  // [B][max_slabs][S * nq] running maximum (base 2) and sum
-  int nq, S, G, row_tiles, max_slabs, fine;
+  int nq, S, G, row_tiles, max_slabs;
+  Slabs slabs;
   int one_round;   // no CTA has a second unit
   unsigned inv_g;  // ceil(2^16 / G): r / G = r * inv_g >> 16 for r < 512, G <= 64
   float scale2;   // scale * log2(e)
@@ -178,9 +183,9 @@ struct SlabList {
 __device__ __forceinline__ SlabList slab_list(const DecodeArgs& a, int len) {
   SlabList s;
   s.lo = a.vis.first(max(0, len - a.S));  // the first key of the oldest row's window
-  s.from = slab_of(s.lo, a.fine);
-  s.first = a.vis.sinks > 0 && s.lo > 0 ? min(slab_of(min(a.vis.sinks, s.lo) - 1, a.fine) + 1, s.from) : 0;
-  s.count = len > 0 ? s.first + slab_of(len - 1, a.fine) + 1 - s.from : 1;  // an empty sequence: one empty slab
+  s.from = a.slabs.of(s.lo);
+  s.first = a.vis.sinks > 0 && s.lo > 0 ? min(a.slabs.of(min(a.vis.sinks, s.lo) - 1) + 1, s.from) : 0;
+  s.count = len > 0 ? s.first + a.slabs.of(len - 1) + 1 - s.from : 1;  // an empty sequence: one empty slab
   return s;
 }
 
@@ -250,8 +255,8 @@ __device__ __noinline__ DecodeUnit decode_unit(const int* s_pre, const int* s_le
   x.lo = sl.lo;
   x.part = slab_g - s_pre[b];
   const int slab = x.part < sl.first ? x.part : sl.from + x.part - sl.first;
-  x.k_begin = slab_begin(slab, a.fine);
-  x.k_end = min(slab_begin(slab + 1, a.fine), x.len);
+  x.k_begin = a.slabs.begin(slab);
+  x.k_end = min(a.slabs.begin(slab + 1), x.len);
   return x;
 }
 
@@ -756,17 +761,16 @@ int paged_check_args(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
   return QMTP_OK;
 }
 
-static bool fine_slabs(int window) { return window > 0 && window <= kFineKeys; }
+static Slabs slabs_for(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
+  return Slabs{c->n_kv < 8 ? 7 : c->n_kv < 16 ? 8 : 9, a->window > 0 && a->window <= kFineKeys};
+}
 
 // Most slabs that one sequence can list: all of its table, or sinks and window with their ragged ends.
 static int max_slabs(const qmtp_paged_args* a, const qmtp_paged_cache* c, int S) {
-  const bool fine = fine_slabs(a->window);
-  const long long cap = (long long)c->table_w * c->page;
-  long long n = slab_of(int(cap - 1), fine) + 1;
-  if (a->window > 0) {
-    const long long k = fine ? kFineSlab : 1;  // fine slabs only: a wide window may cover every slab
-    if (fine) n = std::min(n, (std::min<long long>(a->sinks, cap) + k - 1) / k + (a->window + S + k - 1) / k + 1);
-  }
+  const Slabs sl = slabs_for(a, c);
+  const long long cap = (long long)c->table_w * c->page, k = 1ll << sl.fine_log;
+  long long n = sl.of(int(cap - 1)) + 1;
+  if (sl.all_fine) n = std::min(n, (std::min<long long>(a->sinks, cap) + k - 1) / k + (a->window + S + k - 1) / k + 1);
   return int(n);
 }
 
@@ -869,7 +873,7 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   a.inv_g = (65536 + G - 1) / G;
   a.scale2 = args->scale * kLog2e;
   a.vis = Visible{args->window, args->sinks};
-  a.fine = fine_slabs(args->window);
+  a.slabs = slabs_for(args, cache);
   a.max_slabs = max_slabs(args, cache, S);
   a.err = err;
   a.ws_o = static_cast<float*>(workspace);
