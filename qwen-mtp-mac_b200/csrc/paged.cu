@@ -26,9 +26,7 @@ struct AppendArgs {
   unsigned* err;
 };
 
-constexpr int kAppendSteps = 4;
-
-template <int Dh>
+template <int Dh, int kAppendSteps>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -45,6 +43,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
 #pragma unroll
   for (int i = 0; i < kAppendSteps; ++i) {
     const int h = h0 + i * RPS;
+    x[i] = make_uint4(0, 0, 0, 0);
     if (h < heads) {
       const long long head = h < a.nq ? (a.gated ? 2 * h : h) : (a.gated ? a.nq + h : h);
       x[i] = *reinterpret_cast<const uint4*>(row + head * Dh + 8 * sub);
@@ -72,7 +71,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
     return;
   }
   const int half = a.rotary / 2;
-  float cs[8], sn[8];
+  float cs[8], sn[8];  // the angle's cosine and sine, the sine negative where the partner is taken away
   const int d0 = 8 * sub, i0 = d0 < half ? d0 : d0 - half;
   const bool turns = a.cos_t != nullptr && d0 < a.rotary;
 #pragma unroll
@@ -82,54 +81,49 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
       cv = *reinterpret_cast<const float4*>(a.cos_t + (long long)p * half + i0 + e);
       sv = *reinterpret_cast<const float4*>(a.sin_t + (long long)p * half + i0 + e);
     }
+    const float sign = d0 < half ? -1.0f : 1.0f;
     cs[e] = cv.x; cs[e + 1] = cv.y; cs[e + 2] = cv.z; cs[e + 3] = cv.w;
-    sn[e] = sv.x; sn[e + 1] = sv.y; sn[e + 2] = sv.z; sn[e + 3] = sv.w;
+    sn[e] = sign * sv.x; sn[e + 1] = sign * sv.y; sn[e + 2] = sign * sv.z; sn[e + 3] = sign * sv.w;
   }
   const int lane_p = turns ? lane + (d0 < half ? half / 8 : -(half / 8)) : lane;
-  uint4 wq = make_uint4(0, 0, 0, 0), wk = wq;
-  if (a.qw) wq = *reinterpret_cast<const uint4*>(a.qw + 8 * sub);
-  if (a.kw) wk = *reinterpret_cast<const uint4*>(a.kw + 8 * sub);
+  const long long r0 = cache_row(c, b, 0, p, a.err);  // the position's row of key head 0; a head is a page further
+  const long long head_step = (long long)Dh << c.page_log;
 #pragma unroll
   for (int i = 0; i < kAppendSteps; ++i) {
     const int h = h0 + i * RPS;
     const bool live = h < heads, isq = h < a.nq, isv = h >= a.nq + c.nkv;
-    float y[8];
-    const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { y[2 * e] = live ? bflo(u[e]) : 0.f; y[2 * e + 1] = live ? bfhi(u[e]) : 0.f; }
-    float ss = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = __fmaf_rn(y[e], y[e], ss);
-#pragma unroll
-    for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
-    if ((isq ? a.qw : a.kw) != nullptr) {
-      const float r = rsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / Dh), a.eps));
-      const uint4 w4 = isq ? wq : wk;
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], r), (e & 1) ? bfhi(w[e >> 1]) : bflo(w[e >> 1]));
-    }
-    float o[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_sync(0xFFFFFFFFu, y[e], lane_p);
-      o[e] = y[e];
-      if (turns) o[e] = __fmaf_rn(y[e], cs[e], d0 < half ? -__fmul_rn(other, sn[e]) : __fmul_rn(other, sn[e]));
-    }
-    if (!live) continue;
     uint4 r4 = x[i];
-    if (!isv) {
-      uint32_t pk[4];
+    const uint16_t* weight = isq ? a.qw : a.kw;
+    if (__any_sync(0xFFFFFFFFu, live && !isv)) {  // values are copied as they are
+      float y[8];
+      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pk[e] = f2bf(o[2 * e]) | (uint32_t(f2bf(o[2 * e + 1])) << 16);
-      r4 = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+      for (int e = 0; e < 4; ++e) { y[2 * e] = bflo(u[e]); y[2 * e + 1] = bfhi(u[e]); }
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = __fmaf_rn(y[e], y[e], ss);
+#pragma unroll
+      for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
+      if (weight != nullptr) {
+        const float r = rsqrtf(__fmaf_rn(ss, 1.0f / Dh, a.eps));
+        const uint4 w4 = *reinterpret_cast<const uint4*>(weight + 8 * sub);
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], r), (e & 1) ? bfhi(w[e >> 1]) : bflo(w[e >> 1]));
+      }
+      if (a.cos_t != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float other = __shfl_sync(0xFFFFFFFFu, y[e], lane_p);
+          if (turns) y[e] = __fmaf_rn(y[e], cs[e], __fmul_rn(other, sn[e]));
+        }
+      }
+      if (!isv) r4 = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
     }
-    if (isq) {
+    if (live && isq)
       *reinterpret_cast<uint4*>(a.q_out + ((long long)t * a.nq + h) * Dh + d0) = r4;
-    } else {
-      const long long r = cache_row(c, b, isv ? h - a.nq - c.nkv : h - a.nq, p, a.err);
-      if (r >= 0) *reinterpret_cast<uint4*>((isv ? c.v : c.k) + r * Dh + d0) = r4;
-    }
+    else if (live && r0 >= 0)
+      *reinterpret_cast<uint4*>((isv ? c.v : c.k) + r0 * Dh + (isv ? h - a.nq - c.nkv : h - a.nq) * head_step + d0) = r4;
   }
 }
 
@@ -215,8 +209,8 @@ __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128
 template <int Dh, int NT>
 struct DecodeCfg {
   static constexpr int KG = Dh == 64 ? 2 : 1, TK = 64 * KG;
-  static constexpr int per_sm = Dh == 256 || NT == 4 ? 2 : 3;
-  static constexpr int ring = Dh == 256 ? 3 : NT < 4 ? 4 : 6;  // entries: a tile of K or of V each
+  static constexpr int per_sm = Dh == 256 || (NT == 4 && Dh == 128) ? 2 : 3;
+  static constexpr int ring = Dh == 256 ? 3 : NT < 4 ? 4 : Dh == 128 ? 6 : 3;  // entries: a tile of K or of V each
 };
 
 template <int Dh, int NT>
@@ -802,12 +796,20 @@ static int launch_decode(const PagedView& v, DecodeArgs a, long long units, cuda
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
 }
 
+template <int Dh, int STEPS>
+static int launch_append_steps(const PagedView& v, const AppendArgs& a, cudaStream_t st) {
+  const int per = STEPS * (32 / (Dh / 8));
+  const long long warps = (long long)a.T * ((a.nq + 2 * v.nkv + per - 1) / per);
+  launch_kernel(paged_append_kernel<Dh, STEPS>, dim3(unsigned((warps + 7) / 8)), dim3(256), 0, st, v, a);
+  return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
+}
+
+// Few rows: one a lane group, so that none waits for another (3 tokens of 16 + 8 heads of 256: 2.6 us, with four steps a
+// warp 3.5).  Many: four, which share a token's position and angles (15437 tokens: 84 us, with two 104).
 template <int Dh>
 static int launch_append(const PagedView& v, const AppendArgs& a, cudaStream_t st) {
-  const int per = kAppendSteps * (32 / (Dh / 8));
-  const long long warps = (long long)a.T * ((a.nq + 2 * v.nkv + per - 1) / per);
-  launch_kernel(paged_append_kernel<Dh>, dim3(unsigned((warps + 7) / 8)), dim3(256), 0, st, v, a);
-  return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
+  const long long groups = (long long)a.T * (a.nq + 2 * v.nkv) * Dh / 256;  // warps of one row step
+  return groups < 32ll * sm_count() ? launch_append_steps<Dh, 1>(v, a, st) : launch_append_steps<Dh, 4>(v, a, st);
 }
 
 }  // namespace qmtp

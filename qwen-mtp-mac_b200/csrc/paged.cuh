@@ -37,6 +37,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
 // Length of sequence b: a value the table cannot hold counts as empty (and is reported).
 __device__ __forceinline__ int seq_len(const PagedView& c, int b, unsigned* err) {
   const int n = c.lens[b];
