@@ -12,8 +12,10 @@ namespace qmtp {
 // ----------------------------------------------------------------------------- append
 // Per head row x of q or k: y = x / sqrt(mean x^2 + eps) * w, then dims (i, i + R/2), i < R/2, turn by the
 // position's angle: (y_i c - y_j s, y_j c + y_i s).  All fp32; one rounding to bf16 on the way out.
-// A group of Dh / 8 lanes owns a row (16 bytes a lane); a warp takes 4 steps of 32 / (Dh / 8) head rows of
-// one token, loads all of them first and shares the token's angles.  Bound: HBM (one read, one write).
+// A group of Dh / 8 lanes owns a row.  Of the rotated dims a lane takes four and their four partners (two loads of
+// 8 bytes), so a pair never leaves its lane; of the others, eight in a row.  A warp takes STEPS steps of
+// 32 / (Dh / 8) head rows of one token, loads them all first and shares the token's angles.  Bound: HBM (one read,
+// one write), with the instructions close behind (an early form of 285 a row step took 129 us where this takes 70).
 struct AppendArgs {
   const uint16_t* qkv;
   long long ld;
@@ -26,27 +28,28 @@ struct AppendArgs {
   unsigned* err;
 };
 
-template <int Dh, int kAppendSteps>
+template <int Dh, int STEPS>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendArgs a) {
   pdl_trigger();
   pdl_wait();
   constexpr int LPR = Dh / 8, RPS = 32 / LPR;  // lanes per row, rows per step
-  const int lane = threadIdx.x & 31, sub = lane % LPR;
-  const int heads = a.nq + 2 * c.nkv;
-  const int units = (heads + kAppendSteps * RPS - 1) / (kAppendSteps * RPS);  // warps per token
-  const long long wid = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int t = int(wid / units);
-  const int h0 = int(wid - (long long)t * units) * kAppendSteps * RPS + lane / LPR;
+  const int lane = threadIdx.x & 31, sub = lane % LPR, half = a.rotary / 2;
+  const bool turns = 8 * sub < a.rotary;
+  const int da = turns ? 4 * sub : 8 * sub, db = turns ? half + 4 * sub : 8 * sub + 4;  // this lane's dims: 4 from each on
+  const unsigned heads = a.nq + 2 * c.nkv, units = (heads + STEPS * RPS - 1) / (STEPS * RPS);  // warps per token
+  const unsigned wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int t = wid / units, h0 = (wid - t * units) * STEPS * RPS + lane / LPR;
   if (t >= a.T) return;
   const uint16_t* row = a.qkv + (long long)t * a.ld;
-  uint4 x[kAppendSteps];
+  uint2 x[STEPS][2];
 #pragma unroll
-  for (int i = 0; i < kAppendSteps; ++i) {
+  for (int i = 0; i < STEPS; ++i) {
     const int h = h0 + i * RPS;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (h < heads) {
-      const long long head = h < a.nq ? (a.gated ? 2 * h : h) : (a.gated ? a.nq + h : h);
-      x[i] = *reinterpret_cast<const uint4*>(row + head * Dh + 8 * sub);
+    x[i][0] = x[i][1] = make_uint2(0, 0);
+    if (h < int(heads)) {
+      const uint16_t* src = row + (a.gated ? (h < a.nq ? 2 * h : a.nq + h) : h) * Dh;
+      x[i][0] = *reinterpret_cast<const uint2*>(src + da);
+      x[i][1] = *reinterpret_cast<const uint2*>(src + db);
     }
   }
   // the row's sequence and position
@@ -70,60 +73,72 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
     if (lane == 0) atomicOr(a.err, DEVERR_BADARG);
     return;
   }
-  const int half = a.rotary / 2;
-  float cs[8], sn[8];  // the angle's cosine and sine, the sine negative where the partner is taken away
-  const int d0 = 8 * sub, i0 = d0 < half ? d0 : d0 - half;
-  const bool turns = a.cos_t != nullptr && d0 < a.rotary;
-#pragma unroll
-  for (int e = 0; e < 8; e += 4) {
-    float4 cv = make_float4(1.f, 1.f, 1.f, 1.f), sv = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (turns) {
-      cv = *reinterpret_cast<const float4*>(a.cos_t + (long long)p * half + i0 + e);
-      sv = *reinterpret_cast<const float4*>(a.sin_t + (long long)p * half + i0 + e);
-    }
-    const float sign = d0 < half ? -1.0f : 1.0f;
-    cs[e] = cv.x; cs[e + 1] = cv.y; cs[e + 2] = cv.z; cs[e + 3] = cv.w;
-    sn[e] = sign * sv.x; sn[e + 1] = sign * sv.y; sn[e + 2] = sign * sv.z; sn[e + 3] = sign * sv.w;
+  float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (turns) {
+    cs = *reinterpret_cast<const float4*>(a.cos_t + (long long)p * half + da);
+    sn = *reinterpret_cast<const float4*>(a.sin_t + (long long)p * half + da);
   }
-  const int lane_p = turns ? lane + (d0 < half ? half / 8 : -(half / 8)) : lane;
+  const uint64_t c2[2] = {f2_pack(cs.x, cs.y), f2_pack(cs.z, cs.w)};
+  const uint64_t s2[2] = {f2_pack(sn.x, sn.y), f2_pack(sn.z, sn.w)}, n2[2] = {f2_pack(-sn.x, -sn.y), f2_pack(-sn.z, -sn.w)};
   const long long r0 = cache_row(c, b, 0, p, a.err);  // the position's row of key head 0; a head is a page further
-  const long long head_step = (long long)Dh << c.page_log;
 #pragma unroll
-  for (int i = 0; i < kAppendSteps; ++i) {
+  for (int i = 0; i < STEPS; ++i) {
     const int h = h0 + i * RPS;
-    const bool live = h < heads, isq = h < a.nq, isv = h >= a.nq + c.nkv;
-    uint4 r4 = x[i];
+    const bool live = h < int(heads), isq = h < a.nq, isv = h >= a.nq + c.nkv;
+    uint2 out[2] = {x[i][0], x[i][1]};
     const uint16_t* weight = isq ? a.qw : a.kw;
     if (__any_sync(0xFFFFFFFFu, live && !isv)) {  // values are copied as they are
-      float y[8];
-      const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint64_t y[2][2];
+      uint64_t ss2 = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { y[2 * e] = bflo(u[e]); y[2 * e + 1] = bfhi(u[e]); }
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = __fmaf_rn(y[e], y[e], ss);
-#pragma unroll
-      for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
-      if (weight != nullptr) {
-        const float r = rsqrtf(__fmaf_rn(ss, 1.0f / Dh, a.eps));
-        const uint4 w4 = *reinterpret_cast<const uint4*>(weight + 8 * sub);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(__fmul_rn(y[e], r), (e & 1) ? bfhi(w[e >> 1]) : bflo(w[e >> 1]));
+      for (int k = 0; k < 2; ++k) {
+        y[k][0] = f2_pack(bflo(x[i][k].x), bfhi(x[i][k].x));
+        y[k][1] = f2_pack(bflo(x[i][k].y), bfhi(x[i][k].y));
+        ss2 = f2_fma(y[k][0], y[k][0], ss2);
+        ss2 = f2_fma(y[k][1], y[k][1], ss2);
       }
-      if (a.cos_t != nullptr) {
+      if (weight != nullptr) {
+        float sa, sb;
+        f2_unpack(ss2, sa, sb);
+        float ss = __fadd_rn(sa, sb);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float other = __shfl_sync(0xFFFFFFFFu, y[e], lane_p);
-          if (turns) y[e] = __fmaf_rn(y[e], cs[e], __fmul_rn(other, sn[e]));
+        for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
+        const float r = rsqrtf(__fmaf_rn(ss, 1.0f / Dh, a.eps));
+        const uint64_t r2 = f2_pack(r, r);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint2 w = *reinterpret_cast<const uint2*>(weight + (k ? db : da));
+          y[k][0] = f2_mul(f2_mul(y[k][0], r2), f2_pack(bflo(w.x), bfhi(w.x)));
+          y[k][1] = f2_mul(f2_mul(y[k][1], r2), f2_pack(bflo(w.y), bfhi(w.y)));
         }
       }
-      if (!isv) r4 = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+      if (turns) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint64_t u = y[0][k], v = y[1][k];
+          y[0][k] = f2_fma(u, c2[k], f2_mul(v, n2[k]));
+          y[1][k] = f2_fma(v, c2[k], f2_mul(u, s2[k]));
+        }
+      }
+      if (!isv) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float e[4];
+          f2_unpack(y[k][0], e[0], e[1]);
+          f2_unpack(y[k][1], e[2], e[3]);
+          out[k] = make_uint2(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]));
+        }
+      }
     }
+    uint16_t* dst = nullptr;
     if (live && isq)
-      *reinterpret_cast<uint4*>(a.q_out + ((long long)t * a.nq + h) * Dh + d0) = r4;
+      dst = a.q_out + ((long long)t * a.nq + h) * Dh;
     else if (live && r0 >= 0)
-      *reinterpret_cast<uint4*>((isv ? c.v : c.k) + r0 * Dh + (isv ? h - a.nq - c.nkv : h - a.nq) * head_step + d0) = r4;
+      dst = (isv ? c.v : c.k) + (r0 + ((long long)(isv ? h - a.nq - c.nkv : h - a.nq) << c.page_log)) * Dh;
+    if (dst) {
+      *reinterpret_cast<uint2*>(dst + da) = out[0];
+      *reinterpret_cast<uint2*>(dst + db) = out[1];
+    }
   }
 }
 
@@ -804,8 +819,8 @@ static int launch_append_steps(const PagedView& v, const AppendArgs& a, cudaStre
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
 }
 
-// Few rows: one a lane group, so that none waits for another (3 tokens of 16 + 8 heads of 256: 2.6 us, with four steps a
-// warp 3.5).  Many: four, which share a token's position and angles (15437 tokens: 84 us, with two 104).
+// Few rows: one a lane group, so that none waits for another (3 tokens of 16 + 8 heads of 256: 2.2 us, with four steps a
+// warp 3.5).  Many: four, which share a token's position and angles (15437 tokens: 79 us, with three 87).
 template <int Dh>
 static int launch_append(const PagedView& v, const AppendArgs& a, cudaStream_t st) {
   const long long groups = (long long)a.T * (a.nq + 2 * v.nkv) * Dh / 256;  // warps of one row step
@@ -829,7 +844,7 @@ extern "C" int qmtp_paged_append(const void* qkv, long long ld, int T, const int
   if (cos_t && max_pos < 1) return QMTP_ERR_SHAPE;
   for (const void* p : {qkv, q_w, k_w, (const void*)cos_t, (const void*)sin_t, (const void*)q_out})
     if (p && !aligned16(p)) return QMTP_ERR_ALIGN;
-  if ((long long)T * (n_q + 2 * cache->n_kv) >= (1ll << 33)) return QMTP_ERR_SHAPE;  // the grid stays below 2^31
+  if ((long long)T * (n_q + 2 * cache->n_kv) >= (1ll << 31)) return QMTP_ERR_SHAPE;  // warps are counted in 32 bits
   unsigned* err = device_error_ptr();
   if (!err) return QMTP_ERR_CUDA;
   AppendArgs a{static_cast<const uint16_t*>(qkv), ld, cu, static_cast<const uint16_t*>(q_w),
