@@ -179,6 +179,7 @@ struct DecodeArgs {
   int nq, S, G, row_tiles, max_slabs;
   Slabs slabs;
   int one_round;   // no CTA has a second unit
+  int cluster;     // FUSED: CTAs of a cluster
   unsigned inv_g;  // ceil(2^16 / G): r / G = r * inv_g >> 16 for r < 512, G <= 64
   float scale2;   // scale * log2(e)
   Visible vis;
@@ -237,11 +238,24 @@ struct DecodeSmem {
   __nv_bfloat16 p[8 * NT][Cfg::TK + 8];  // weights, [row][key]
   float mx[4][8 * NT];
   float sum[2][4][8 * NT];
+  float2 ml[8 * NT];  // FUSED: this slab's maxima and sums
   uint64_t full[Cfg::ring], empty[Cfg::ring], q_full[2], q_empty[2];
   int bad[2];
   int scan[8];
   int dead;
 };
+
+__device__ __forceinline__ float join_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M)); }
+// Four dims of a finished row: sum / denominator, the gate, one rounding.
+__device__ __forceinline__ void join_store(const DecodeArgs& a, float (&y)[4], float ll, uint2 gate, uint16_t* dst) {
+  const float g[4] = {bflo(gate.x), bfhi(gate.x), bflo(gate.y), bfhi(gate.y)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    y[k] = ll == 0.0f ? 0.0f : __fdiv_rn(y[k], ll);
+    if (a.gate) y[k] = __fmul_rn(y[k], sigmoid_f32(g[k]));
+  }
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+}
 
 struct DecodeUnit {
   int b, kh, row0, len, lo, k_begin, k_end, part;
@@ -269,11 +283,14 @@ __device__ __noinline__ DecodeUnit decode_unit(const int* s_pre, const int* s_le
   return x;
 }
 
-template <int Dh, int NT>
+// FUSED: one launch for short tables.  The slabs of a (sequence, key head, row tile) are the CTAs of a cluster, one unit
+// each; their partial results stay in shared memory and every CTA joins its share of the rows' dims through
+// distributed shared memory, in the join kernels' order.
+template <int Dh, int NT, bool FUSED>
 __global__ void __launch_bounds__(160, DecodeCfg<Dh, NT>::per_sm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, PagedView c,
                     const __grid_constant__ DecodeArgs a) {
-  if (a.one_round) pdl_trigger();  // otherwise when the last unit is done: a waiting successor's blocks take up room
+  if (FUSED || a.one_round) pdl_trigger();  // otherwise when the last unit is done: a waiting successor's blocks take up room
   extern __shared__ uint8_t smem_raw[];
   using Smem = DecodeSmem<Dh, NT>;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -291,23 +308,42 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     fence_mbar_init();
   }
   pdl_wait();
-  int total = 0;
-  for (int b0 = 0; b0 < c.B; b0 += 160) {
-    const int b = b0 + tid;
-    int n = 0, len = 0;
-    if (b < c.B) {
-      len = seq_len(c, b, blockIdx.x == 0 ? a.err : nullptr);
-      n = slab_list(a, len).count;
+  const int R = a.S * a.G, per = c.nkv * a.row_tiles;
+  int units = 1;
+  DecodeUnit mine;      // FUSED: the CTA's unit
+  SlabList mine_slabs;
+  if (FUSED) {
+    const int rank = cluster_rank(), cl = blockIdx.x / a.cluster, rest = cl % per;
+    mine.b = cl / per;
+    mine.kh = rest / a.row_tiles;
+    mine.row0 = (rest - mine.kh * a.row_tiles) * 8 * NT;
+    mine.len = seq_len(c, mine.b, rank == 0 ? a.err : nullptr);
+    mine_slabs = slab_list(a, mine.len);
+    mine.lo = mine_slabs.lo;
+    mine.part = rank;
+    const int slab = rank < mine_slabs.first ? rank : mine_slabs.from + rank - mine_slabs.first;
+    mine.k_begin = rank < mine_slabs.count ? a.slabs.begin(slab) : 0;
+    mine.k_end = rank < mine_slabs.count ? min(a.slabs.begin(slab + 1), mine.len) : 0;
+  } else {
+    int total = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 160) {
+      const int b = b0 + tid;
+      int n = 0, len = 0;
+      if (b < c.B) {
+        len = seq_len(c, b, blockIdx.x == 0 ? a.err : nullptr);
+        n = slab_list(a, len).count;
+      }
+      int chunk;
+      const int before = block_excl_scan(n, sm.scan, chunk);
+      if (b < c.B) { s_pre[b] = total + before; s_len[b] = len; }
+      total += chunk;
     }
-    int chunk;
-    const int before = block_excl_scan(n, sm.scan, chunk);
-    if (b < c.B) { s_pre[b] = total + before; s_len[b] = len; }
-    total += chunk;
+    if (tid == 0) s_pre[c.B] = total;
+    units = total * per;
   }
-  if (tid == 0) s_pre[c.B] = total;
   __syncthreads();
-  const int R = a.S * a.G, per = c.nkv * a.row_tiles, units = total * per;
-  auto unit_at = [&](int u) { return decode_unit(s_pre, s_len, a, c.B, c.nkv, 8 * NT, u); };
+  const int u0 = FUSED ? 0 : blockIdx.x, ustep = FUSED ? 1 : gridDim.x;
+  auto unit_at = [&](int u) { return FUSED ? mine : decode_unit(s_pre, s_len, a, c.B, c.nkv, 8 * NT, u); };
   // the next tile of the unit, from key j on, that holds a needed key
   auto next_tile = [&](const DecodeUnit& x, int j) {
     while (j < x.k_end && a.vis.window != 0 && j + kTile <= x.lo && j >= a.vis.sinks) j += kTile;
@@ -340,7 +376,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       ++e;
     };
     DecodeUnit x;
-    int j = 0, row = 0, u = blockIdx.x;
+    int j = 0, row = 0, u = u0;
     if (u < units) {
       x = unit_at(u);
       j = next_tile(x, x.k_begin);
@@ -352,7 +388,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       DecodeUnit xn = x;
       int un = u, jn = j < x.k_end ? next_tile(x, j + kTile) : x.k_end;
       if (jn >= x.k_end) {
-        un = u + gridDim.x;
+        un = u + ustep;
         if (un < units) {
           xn = unit_at(un);
           jn = next_tile(xn, xn.k_begin);
@@ -385,13 +421,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       for (int i = max(0, e - RING); i < e; ++i) mbar_wait_bounded(&sm.full[i % RING], (i / RING) & 1, a.err, 1u << 22);
       for (int i = max(0, uq - QS); i < uq; ++i) mbar_wait_bounded(&sm.q_full[i % QS], (i / QS) & 1, a.err, 1u << 22);
     }
-    return;
+    if (!FUSED) return;
+    __syncwarp();
   }
 
   // ---------------------------------------------------------------------- consumers
   const int quad = lane & 3, oct = lane >> 2;
   int e = 0, uq = 0;
-  for (int u = blockIdx.x; u < units; u += gridDim.x, ++uq) {
+  for (int u = warp == 4 ? units : u0; u < units; u += ustep, ++uq) {
     const DecodeUnit x = unit_at(u);
     const int pos0 = x.len - a.S, set = uq & 1;
     int prow[NT][2];  // positions of this lane's rows n = 8 t + 2 quad + i
@@ -540,7 +577,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.q_empty[uq % QS]);
-    if (u + int(gridDim.x) >= units) pdl_trigger();
+    if (!FUSED && u + ustep >= units) pdl_trigger();
     // sums over the key lanes and warps; is the numerator finite?
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -566,15 +603,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         for (int i = 0; i < 2; ++i) {
           const int n = 8 * t + 2 * quad + i, r = x.row0 + n, s = r * a.inv_g >> 16;
           if (r >= R) continue;
-          const long long at = (part + s) * a.nq + x.kh * a.G + r - s * a.G;
-          float* dst = a.ws_o + at * Dh + warp * MT * 16 + oct;
+          const long long at = FUSED ? n : (part + s) * a.nq + x.kh * a.G + r - s * a.G;
+          float* dst = (FUSED ? reinterpret_cast<float*>(sm.kv) : a.ws_o) + at * Dh + warp * MT * 16 + oct;
 #pragma unroll
           for (int y = 0; y < MT; ++y) {
             dst[16 * y] = o[y][t][i];
             dst[16 * y + 8] = o[y][t][i + 2];
           }
           if (warp == 0 && oct == 0)
-            a.ws_ml[at] = make_float2(m[t][i], __fadd_rn(__fadd_rn(sm.sum[set][0][n], sm.sum[set][1][n]),
+            (FUSED ? sm.ml : a.ws_ml)[at] = make_float2(m[t][i], __fadd_rn(__fadd_rn(sm.sum[set][0][n], sm.sum[set][1][n]),
                                                          __fadd_rn(sm.sum[set][2][n], sm.sum[set][3][n])));
         }
       __syncwarp();
@@ -586,11 +623,70 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         float mm = kNone, ll = 0.0f, oo[Dh / 32] = {};
         attend_row_strict<Dh>(c, a.q + (long long)(x.b * a.S + s) * a.q_ld + (long long)h * Dh, x.b, x.kh, pos0 + s,
                               x.k_begin, x.k_end, a.vis, a.scale2, a.err, mm, ll, oo);
-        const long long at = (part + s) * a.nq + h;
-        for (int i = 0; i < Dh / 32; ++i) a.ws_o[at * Dh + lane * (Dh / 32) + i] = oo[i];
-        if (lane == 0) a.ws_ml[at] = make_float2(mm, ll);
+        const long long at = FUSED ? n : (part + s) * a.nq + h;
+        float* dst = (FUSED ? reinterpret_cast<float*>(sm.kv) : a.ws_o) + at * Dh;
+        for (int i = 0; i < Dh / 32; ++i) dst[lane * (Dh / 32) + i] = oo[i];
+        if (lane == 0) (FUSED ? sm.ml : a.ws_ml)[at] = make_float2(mm, ll);
       }
     }
+  }
+  if (FUSED) {
+    __syncwarp();
+    cluster_sync_all();  // every slab's numerators and (maximum, sum) can be read
+    const int rows = min(8 * NT, R - mine.row0), n_parts = mine_slabs.count;
+    for (int i = mine.part * 160 + tid; i < rows * (Dh / 4); i += a.cluster * 160) {
+      const int n = i / (Dh / 4), d = (i - n * (Dh / 4)) * 4;
+      const int r = mine.row0 + n, s = r * a.inv_g >> 16, h = mine.kh * a.G + r - s * a.G;
+      const long long t = mine.b * a.S + s;
+      uint2 g2 = make_uint2(0, 0);
+      if (a.gate) g2 = *reinterpret_cast<const uint2*>(a.gate + t * a.gate_ld + h * a.gate_hs + d);
+      const float* mlp = reinterpret_cast<const float*>(&sm.ml[n]);
+      const float* op = reinterpret_cast<const float*>(sm.kv) + n * Dh + d;
+      // class k: slab number k of the first ones (few calls have any), and the one of the others with that residue
+      float m1[16], l1[16];
+      int part_of[16];
+      float M = kNone;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int pt = mine_slabs.first + ((k - mine_slabs.from) & 15);
+        part_of[k] = pt < n_parts ? pt : 0;
+        m1[k] = ld_dsmem(mlp, part_of[k]);
+        l1[k] = ld_dsmem(mlp + 1, part_of[k]);
+        if (pt >= n_parts) m1[k] = kNone;
+        M = fmaxf(M, m1[k]);
+      }
+      for (int k = 0; k < mine_slabs.first; ++k) M = fmaxf(M, ld_dsmem(mlp, k));
+      float y[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.0f;
+#pragma unroll
+      for (int k0 = 0; k0 < 16; k0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = ld_dsmem_v4(op, part_of[k0 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float z[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.0f;
+          if (k0 + k < mine_slabs.first) {
+            const float w = join_weight(ld_dsmem(mlp, k0 + k), M);
+            const float4 u = ld_dsmem_v4(op, k0 + k);
+            den = __fmaf_rn(w, ld_dsmem(mlp + 1, k0 + k), den);
+            z[0] = __fmaf_rn(w, u.x, z[0]);
+            z[1] = __fmaf_rn(w, u.y, z[1]);
+            z[2] = __fmaf_rn(w, u.z, z[2]);
+            z[3] = __fmaf_rn(w, u.w, z[3]);
+          }
+          const float w = join_weight(m1[k0 + k], M);
+          den = __fmaf_rn(w, l1[k0 + k], den);
+          y[0] = __fadd_rn(y[0], __fmaf_rn(w, v[k].x, z[0]));
+          y[1] = __fadd_rn(y[1], __fmaf_rn(w, v[k].y, z[1]));
+          y[2] = __fadd_rn(y[2], __fmaf_rn(w, v[k].z, z[2]));
+          y[3] = __fadd_rn(y[3], __fmaf_rn(w, v[k].w, z[3]));
+          ll = __fadd_rn(ll, den);
+        }
+      }
+      join_store(a, y, ll, g2, a.out + (t * a.nq + h) * Dh + d);
+    }
+    __syncwarp();
+    cluster_sync_all();  // the others have read this CTA's shared memory
   }
 }
 
@@ -618,7 +714,6 @@ __device__ __forceinline__ JoinRow join_row(const PagedView& c, const DecodeArgs
   j.gate = t * a.gate_ld + h * a.gate_hs;
   return j;
 }
-__device__ __forceinline__ float join_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M)); }
 
 template <int Dh>
 __global__ void __launch_bounds__(256) paged_join_wide_kernel(PagedView c, DecodeArgs a) {
@@ -732,15 +827,7 @@ __global__ void __launch_bounds__(128) paged_join_warp_kernel(PagedView c, Decod
     y[3] = __fadd_rn(y[3], acc[k].w);
     ll = __fadd_rn(ll, __shfl_sync(0xFFFFFFFFu, den, half + k));
   }
-  const float g[4] = {bflo(g2.x), bfhi(g2.x), bflo(g2.y), bfhi(g2.y)};
-  uint16_t h[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    y[k] = ll == 0.0f ? 0.0f : __fdiv_rn(y[k], ll);
-    if (a.gate) y[k] = __fmul_rn(y[k], sigmoid_f32(g[k]));
-    h[k] = f2bf(y[k]);
-  }
-  if (live) *reinterpret_cast<uint2*>(a.out + j.out + d) = make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
+  if (live) join_store(a, y, ll, g2, a.out + j.out + d);
 }
 
 // ----------------------------------------------------------------------------- host
@@ -783,6 +870,19 @@ static int max_slabs(const qmtp_paged_args* a, const qmtp_paged_cache* c, int S)
   return int(n);
 }
 
+// Rows of a tile, in groups of 8: as many as there are up to 32, at 256 dims up to 16 (registers); K and V are read
+// once a tile.
+static int row_groups(int rows, int Dh) { return rows <= 8 ? 1 : rows <= 16 || Dh == 256 ? 2 : 4; }
+
+// CTAs of a cluster when the call fits the fused form, else 0: a table of at most 16 slabs, and clusters that fill no
+// more than one CTA per SM.  Measured (4 key heads of 256, 4 rows): 515 keys 7.7 us fused, 8.7 with the
+// join as a second launch.
+static int fused_cluster(const qmtp_paged_args* a, const qmtp_paged_cache* c, int S) {
+  const int n = max_slabs(a, c, S), rows = S * (a->n_q / c->n_kv), per_tile = 8 * row_groups(rows, c->Dh);
+  const int cluster = n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
+  return n <= 16 && (long long)c->B * c->n_kv * ((rows + per_tile - 1) / per_tile) * cluster <= sm_count() ? cluster : 0;
+}
+
 static size_t align_up(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <int Dh, int NT>
@@ -790,17 +890,29 @@ static int launch_decode(const PagedView& v, DecodeArgs a, long long units, cuda
   constexpr size_t fixed = sizeof(DecodeSmem<Dh, NT>) + 1024;
   static DeviceOnce ready;
   if (!ready([] {
-        return cudaFuncSetAttribute(paged_decode_kernel<Dh, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    int(fixed + (2 * kMaxSeqs + 1) * sizeof(int)));
+        if (const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<Dh, NT, false>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       int(fixed + (2 * kMaxSeqs + 1) * sizeof(int))))
+          return e;
+        if (const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<Dh, NT, true>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, int(fixed)))
+          return e;
+        return cudaFuncSetAttribute(paged_decode_kernel<Dh, NT, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
       }))
     return QMTP_ERR_CUDA;
   CUtensorMap tk, tv;
   const cuuint64_t kd[2] = {Dh, cuuint64_t((v.pages * v.nkv) << v.page_log)}, ks[1] = {Dh * 2};
   const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, DecodeCfg<Dh, NT>::TK))};
   if (!encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb)) return QMTP_ERR_CUDA;
+  if (a.cluster) {
+    const int grid = v.B * v.nkv * a.row_tiles * a.cluster;
+    launch_kernel_cluster(paged_decode_kernel<Dh, NT, true>, dim3(grid), dim3(160), fixed, st, a.cluster, tk, tv, v, a);
+    return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
+  }
   const int grid = int(std::min<long long>(units, (long long)sm_count() * DecodeCfg<Dh, NT>::per_sm));
   a.one_round = grid == units;
-  launch_kernel(paged_decode_kernel<Dh, NT>, dim3(grid), dim3(160), fixed + (2 * v.B + 1) * sizeof(int), st, tk, tv, v, a);
+  launch_kernel(paged_decode_kernel<Dh, NT, false>, dim3(grid), dim3(160), fixed + (2 * v.B + 1) * sizeof(int), st, tk, tv, v,
+                a);
   const int rows = v.B * a.S * a.nq;
   if (rows >= 2 * sm_count()) {
     constexpr int RPW = Dh == 64 ? 2 : 1, WPR = Dh == 256 ? 2 : 1;
@@ -859,6 +971,7 @@ extern "C" size_t qmtp_paged_attention_workspace(const qmtp_paged_args* args, co
   PagedView v;
   if (paged_view(cache, &v) || paged_check_args(args, cache)) return 0;
   const int S = args->T / cache->B, n = max_slabs(args, cache, S);
+  if (fused_cluster(args, cache, S)) return 0;
   const size_t rows = size_t(cache->B) * n * S * args->n_q;
   return align_up(rows * cache->Dh * sizeof(float)) + rows * sizeof(float2);
 }
@@ -872,9 +985,9 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   const int S = args->T / v.B, G = args->n_q / v.nkv;
   if (S > kMaxS) return QMTP_ERR_UNSUPPORTED;
   const size_t need = qmtp_paged_attention_workspace(args, cache);
-  if (!workspace) return QMTP_ERR_ARG;
+  if (need && !workspace) return QMTP_ERR_ARG;
   if (ws_bytes < need) return QMTP_ERR_SHAPE;
-  if (!aligned16(workspace)) return QMTP_ERR_ALIGN;
+  if (need && !aligned16(workspace)) return QMTP_ERR_ALIGN;
   unsigned* err = device_error_ptr();
   if (!err) return QMTP_ERR_CUDA;
   DecodeArgs a{};
@@ -892,12 +1005,12 @@ extern "C" int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_page
   a.vis = Visible{args->window, args->sinks};
   a.slabs = slabs_for(args, cache);
   a.max_slabs = max_slabs(args, cache, S);
+  a.cluster = fused_cluster(args, cache, S);
   a.err = err;
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) +
                                       align_up(size_t(v.B) * a.max_slabs * S * a.nq * cache->Dh * sizeof(float)));
-  // rows of a tile: as many as there are up to 32, at 256 dims up to 16 (registers); K and V are read once a tile
-  const int nt = S * G <= 8 ? 1 : S * G <= 16 || cache->Dh == 256 ? 2 : 4;
+  const int nt = row_groups(S * G, cache->Dh);
   a.row_tiles = (S * G + 8 * nt - 1) / (8 * nt);
   const long long units = (long long)v.B * a.max_slabs * v.nkv * a.row_tiles;
   if (units >= (1ll << 30) || (long long)v.B * S * a.nq >= (1ll << 28)) return QMTP_ERR_SHAPE;

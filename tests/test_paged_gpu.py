@@ -307,3 +307,25 @@ def test_decode_in_a_graph_follows_the_device_state(dev):
         got = out.clone()
         assert torch.equal(got, step()), i
     no_error()
+
+
+@pytest.mark.parametrize("nq,nkv,dh,S", [(16, 4, 256, 1), (16, 4, 256, 3), (8, 2, 128, 1), (14, 2, 128, 2), (16, 2, 128, 4),
+                                         (4, 4, 64, 1), (8, 1, 64, 2), (8, 1, 64, 4)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 4), (129, 200)])
+def test_decode_one_launch_and_two_give_the_same_bits(nq, nkv, dh, S, window, sinks, dev):
+    """Short tables run as one launch (the slabs of a row in a thread-block cluster), wide ones as two: a table row with
+    spare entries at its end takes the other way over the same keys."""
+    from qmtp import paged
+
+    for length in (1, 128, 515, 1000, 2048):
+        if length < S:
+            continue
+        bt = Batch([(S, length)], nq, nkv, dh, 64, seed=length + S).put(dev)
+        q, cache, table, lens = bt.args()
+        wide = torch.full((1, 1000), -1, dtype=torch.int32, device=dev)
+        wide[:, : table.shape[1]] = table
+        kw = dict(gate=bt.d["gate"][:, :, 1], window=window, sinks=sinks)
+        one, two = paged.attention(q, cache, table, lens, **kw), paged.attention(q, cache, wide, lens, **kw)
+        no_error()
+        assert torch.equal(one, two), length
+        check(one, attention_ref(bt, window, sinks))
