@@ -42,6 +42,7 @@ struct PromptArgs {
   float* ws_o;    // [splits][T][nq][Dh]
   float2* ws_ml;  // [splits][T][nq]
   int T, nq, G, tpt, splits;  // tpt: tokens per row tile
+  int takes_over;             // more blocks than SMs
   float scale2;
   Visible vis;
   unsigned* err;
@@ -242,8 +243,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     int e0 = 0, issued = 0, loads = 0;
     long long u = blockIdx.x;
     for (int i = 0;; ++i) {
-      // the next item: that of a block of the grid that has not started, taken over while this one runs
-      if (lane == 0) {
+      // The next item: that of a block of the grid that has not started, taken over while this one runs.  With no more
+      // blocks than SMs each finds a place of its own, and none is taken.
+      if (lane == 0 && a.takes_over) {
         mbar_expect_tx(&bars->next_full, 16);
         next_block_request(bars->next, &bars->next_full);
       }
@@ -351,7 +353,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         e0 += 2 * ts.nt * E;
       }
       int next = -1;
-      if (bar_wait(&bars->dead, &bars->next_full, i & 1, a.err)) next = next_block(bars->next);
+      if (a.takes_over && bar_wait(&bars->dead, &bars->next_full, i & 1, a.err)) next = next_block(bars->next);
       next = __shfl_sync(0xFFFFFFFFu, next, 0);
       if (x.b < 0 || !ok) break;
       if (next < 0) {
@@ -711,7 +713,7 @@ static int prompt_splits(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
 }
 
 template <int Dh>
-static int launch_prompt(const qmtp_paged_args* args, const PagedView& v, const PromptArgs& a, long long items,
+static int launch_prompt(const qmtp_paged_args* args, const PagedView& v, PromptArgs a, long long items,
                          cudaStream_t st) {
   using Cfg = PromptCfg<Dh>;
   static DeviceOnce ready;
@@ -726,6 +728,7 @@ static int launch_prompt(const qmtp_paged_args* args, const PagedView& v, const 
   const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kKeys / Cfg::E))};
   if (!encode_pages(&tq, a.q, 3, qd, qs, qb) || !encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb))
     return QMTP_ERR_CUDA;
+  a.takes_over = items * a.splits > sm_count();
   launch_kernel(paged_prompt_kernel<Dh>, dim3(unsigned(items * a.splits)), dim3(Cfg::threads), Cfg::smem, st, tq, tk, tv, v, a);
   if (a.splits > 1)
     launch_kernel(prompt_join_kernel<Dh>, dim3(unsigned(((long long)a.T * a.nq + 7) / 8)), dim3(256), 0, st, v, a);
