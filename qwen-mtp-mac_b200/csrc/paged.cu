@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(128) paged_join_warp_kernel(PagedView c, Decod
 // ----------------------------------------------------------------------------- host
 int paged_view(const qmtp_paged_cache* c, PagedView* v) {
   if (!c || !c->k || !c->v || !c->table || !c->lens) return QMTP_ERR_ARG;
-  if (c->B < 1 || c->B > kMaxSeqs || c->n_kv < 1 || c->pages < 1 || c->table_w < 1 || c->ld_table < c->table_w)
+  if (c->B < 1 || c->B > kMaxSeqs || c->n_kv < 1 || c->n_kv > kMaxHeads || c->pages < 1 || c->table_w < 1 || c->ld_table < c->table_w)
     return QMTP_ERR_SHAPE;
   if (c->Dh != 64 && c->Dh != 128 && c->Dh != 256) return QMTP_ERR_UNSUPPORTED;
   if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1))) return QMTP_ERR_UNSUPPORTED;
@@ -849,7 +849,7 @@ int paged_view(const qmtp_paged_cache* c, PagedView* v) {
 int paged_check_args(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
   if (!a || !a->q || !a->out) return QMTP_ERR_ARG;
   if (!(a->scale > 0.0f) || !std::isfinite(a->scale) || a->window < 0 || a->sinks < 0) return QMTP_ERR_ARG;
-  if (a->T < 1 || a->n_q < 1 || a->n_q % c->n_kv) return QMTP_ERR_SHAPE;
+  if (a->T < 1 || a->n_q < 1 || a->n_q > kMaxHeads || a->n_q % c->n_kv) return QMTP_ERR_SHAPE;
   if (a->n_q / c->n_kv > 64) return QMTP_ERR_UNSUPPORTED;
   if (a->q_ld % 8 || (a->q_ld && a->q_ld < (long long)a->n_q * c->Dh)) return QMTP_ERR_SHAPE;
   if (a->gate && (a->gate_ld % 8 || a->gate_hs % 8)) return QMTP_ERR_SHAPE;
@@ -949,7 +949,7 @@ extern "C" int qmtp_paged_append(const void* qkv, long long ld, int T, const int
   PagedView v;
   if (const int rc = paged_view(cache, &v)) return rc;
   if (!qkv || !q_out || (cos_t == nullptr) != (sin_t == nullptr) || !(eps >= 0.0f)) return QMTP_ERR_ARG;
-  if (T < 1 || n_q < 1 || ld % 8 || ld < (long long)(n_q * (gated ? 2 : 1) + 2 * cache->n_kv) * cache->Dh)
+  if (T < 1 || n_q < 1 || n_q > kMaxHeads || ld % 8 || ld < (long long)(n_q * (gated ? 2 : 1) + 2 * cache->n_kv) * cache->Dh)
     return QMTP_ERR_SHAPE;
   if (!cu && T % cache->B) return QMTP_ERR_SHAPE;
   if (cos_t && (rotary < 16 || rotary > cache->Dh || rotary % 16)) return QMTP_ERR_UNSUPPORTED;

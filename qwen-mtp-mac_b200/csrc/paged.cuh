@@ -10,6 +10,7 @@ namespace qmtp {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kMaxSeqs = 4096;
+constexpr int kMaxHeads = 65536;
 
 // Device view of qmtp_paged_cache.  page = 1 << page_log.
 struct PagedView {

@@ -23,6 +23,7 @@ from . import _lib
 
 MAX_NEW = 8  # new tokens per sequence that ``attention`` takes
 BF16 = torch.bfloat16
+_INT_MAX = 2 ** 31 - 1
 
 
 class PagedCache:
@@ -160,16 +161,18 @@ def _attention_args(q, cache: PagedCache, gate, scale, window, sinks, out):
     _tensor("q", q, BF16, dev)
     if q.dim() != 3 or q.shape[2] != dh:
         _need(False, "q is [rows, heads, head_dim]")
-    (T, nq, _), (_, hs, one) = q.shape, q.stride()
-    if nq < 1 or one != 1 or (hs != dh and nq > 1):
-        _need(False, "a row of q needs to be contiguous")
+    (T, nq, _), (ld, hs, one) = q.shape, q.stride()
+    if nq < 1 or one != 1 or (hs != dh and nq > 1) or (ld < nq * dh and T > 1):
+        _need(False, "a row of q needs to be contiguous, and rows apart")
+    if window < 0 or sinks < 0:
+        _need(False, "window and sinks count tokens")
     if out is None:
         out = q.new_empty((T, nq * dh))
     else:
         _tensor("out", out, BF16, dev)
         _need(out.shape == (T, nq * dh) and out.is_contiguous(), "out is [rows, heads * head_dim], contiguous")
     a = _lib.PagedArgs(q.data_ptr(), None, out.data_ptr(), _row_stride(q, nq * dh), 0, 0, T, nq,
-                       dh ** -0.5 if scale is None else scale, window, sinks)
+                       dh ** -0.5 if scale is None else scale, min(window, _INT_MAX), min(sinks, _INT_MAX))
     if gate is not None:
         _tensor("gate", gate, BF16, dev)
         ld, hs, one = gate.stride() if gate.dim() == 3 else (0, 0, 0)

@@ -27,14 +27,14 @@ def attn(**kw):
 
 BAD_CACHE = [
     (dict(k=None), ARG), (dict(v=None), ARG), (dict(table=None), ARG), (dict(lens=None), ARG), (dict(B=0), SHAPE),
-    (dict(B=4097), SHAPE), (dict(n_kv=0), SHAPE), (dict(pages=0), SHAPE), (dict(table_w=0), SHAPE),
+    (dict(B=4097), SHAPE), (dict(n_kv=0), SHAPE), (dict(n_kv=65537), SHAPE), (dict(pages=0), SHAPE), (dict(table_w=0), SHAPE),
     (dict(ld_table=3), SHAPE), (dict(Dh=96), UNSUPPORTED), (dict(Dh=512), UNSUPPORTED), (dict(page=8), UNSUPPORTED),
     (dict(page=48), UNSUPPORTED), (dict(page=512), UNSUPPORTED), (dict(pages=1 << 27), SHAPE),
     (dict(table_w=1 << 28, ld_table=1 << 28), SHAPE), (dict(k=PTR + 8), ALIGN), (dict(v=PTR + 2), ALIGN)]
 BAD_ATTN = [
     (dict(q=None), ARG), (dict(out=None), ARG), (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG),
     (dict(scale=float("nan")), ARG), (dict(scale=float("inf")), ARG), (dict(window=-1), ARG), (dict(sinks=-1), ARG),
-    (dict(T=0), SHAPE), (dict(n_q=0), SHAPE), (dict(n_q=5), SHAPE), (dict(n_q=130), UNSUPPORTED), (dict(q_ld=4), SHAPE),
+    (dict(T=0), SHAPE), (dict(n_q=0), SHAPE), (dict(n_q=5), SHAPE), (dict(n_q=1 << 30), SHAPE), (dict(n_q=130), UNSUPPORTED), (dict(q_ld=4), SHAPE),
     (dict(q_ld=504), SHAPE), (dict(gate=PTR, gate_ld=12), SHAPE), (dict(gate=PTR, gate_hs=4), SHAPE),
     (dict(q=PTR + 8), ALIGN), (dict(out=PTR + 2), ALIGN), (dict(gate=PTR + 2), ALIGN)]
 
@@ -83,7 +83,7 @@ def test_attention_workspace():
 
 @pytest.mark.parametrize("change,code", [
     (dict(qkv=None), ARG), (dict(q_out=None), ARG), (dict(cos=PTR), ARG), (dict(eps=-1.0), ARG), (dict(eps=float("nan")), ARG),
-    (dict(T=0), SHAPE), (dict(T=3), SHAPE), (dict(n_q=0), SHAPE), (dict(ld=1020), SHAPE), (dict(ld=1016), SHAPE),
+    (dict(T=0), SHAPE), (dict(T=3), SHAPE), (dict(n_q=0), SHAPE), (dict(n_q=1 << 30), SHAPE), (dict(ld=1020), SHAPE), (dict(ld=1016), SHAPE),
     (dict(gated=1), SHAPE), (dict(cos=PTR, sin=PTR, rotary=24, max_pos=9), UNSUPPORTED),
     (dict(cos=PTR, sin=PTR, rotary=144, max_pos=9), UNSUPPORTED), (dict(cos=PTR, sin=PTR, rotary=0, max_pos=9), UNSUPPORTED),
     (dict(cos=PTR, sin=PTR, rotary=32, max_pos=0), SHAPE), (dict(qkv=PTR + 2), ALIGN), (dict(q_out=PTR + 8), ALIGN),

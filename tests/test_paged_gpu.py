@@ -329,3 +329,114 @@ def test_decode_one_launch_and_two_give_the_same_bits(nq, nkv, dh, S, window, si
         no_error()
         assert torch.equal(one, two), length
         check(one, attention_ref(bt, window, sinks))
+
+
+def test_most_sequences(dev):
+    """4096 sequences, the most a call takes: append, decode and prompt attention of one new token each."""
+    from qmtp import paged
+
+    bt = Batch([(1, 1 + i % 37) for i in range(4096)], 2, 1, 64, 16, seed=9).put(dev)
+    ref = attention_ref(bt, gate=False)
+    check(paged.attention(*bt.args()), ref)
+    check(paged.prompt_attention(*bt.args(), bt.d["cu"]), ref)
+    qkv = torch.randn((4096, 4 * 64), device=dev).to(BF16)
+    q, _ = paged.append_qkv(qkv, bt.cache, bt.d["table"], bt.d["lens"], bt.d["cu"], n_heads=2)
+    no_error()
+    assert torch.equal(q, qkv[:, :128].reshape(4096, 2, 64))
+    pg = bt.d["table"].long().gather(1, ((bt.d["lens"].long() - 1) // 16)[:, None])[:, 0]
+    assert torch.equal(bt.cache.v[pg, 0, (bt.d["lens"].long() - 1) % 16], qkv[:, 192:])
+
+
+def test_shared_pages(dev):
+    """Two sequences that begin with the same pages (a shared prompt) and end on their own."""
+    from qmtp import paged
+
+    bt = Batch([(2, 100), (2, 90)], 4, 2, 128, 16, seed=10)
+    bt.table[1, :4] = bt.table[0, :4]
+    bt.put(dev)
+    ref = attention_ref(bt)
+    kw = dict(gate=bt.d["gate"][:, :, 1])
+    check(paged.attention(*bt.args(), **kw), ref)
+    check(paged.prompt_attention(*bt.args(), bt.d["cu"], **kw), ref)
+    no_error()
+
+
+def test_two_streams_at_once(dev):
+    """Calls of one cache on two streams, each with its own workspace, many times."""
+    from qmtp import paged
+
+    bt = Batch([(3, 5000), (3, 3000)], 16, 4, 256, 64, seed=11).put(dev)
+    other = bt.d["q"].flip(0).contiguous()
+    want = [(paged.attention(q, *bt.args()[1:]), paged.prompt_attention(q, *bt.args()[1:], bt.d["cu"])) for q in (bt.d["q"], other)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, q in enumerate((bt.d["q"], other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((paged.attention(q, *bt.args()[1:]), paged.prompt_attention(q, *bt.args()[1:], bt.d["cu"])))
+    no_error()
+    for i in range(2):
+        assert all(torch.equal(a, want[i][0]) and torch.equal(b, want[i][1]) for a, b in got[i])
+
+
+def test_broadcast_gate_and_huge_window(dev):
+    """One gate row for all tokens (stride 0); a window beyond every position is no window's values."""
+    from qmtp import paged
+
+    bt = Batch([(2, 70)], 4, 2, 64, 16, seed=12)
+    bt.gate[:] = bt.gate[:1]
+    bt.put(dev)
+    gate = bt.d["gate"][:1, :, 1].expand(2, 4, 64)
+    for f in (paged.attention, lambda *a, **k: paged.prompt_attention(*a, bt.d["cu"], **k)):
+        check(f(*bt.args(), gate=gate, window=2 ** 40, sinks=2 ** 33), attention_ref(bt))
+    no_error()
+
+
+def test_python_refusals(dev):
+    from qmtp import paged
+
+    bt = Batch([(2, 70), (2, 40)], 4, 2, 64, 16, seed=13).put(dev)
+    q, cache, table, lens = bt.args()
+    cu = bt.d["cu"]
+    bad = [dict(q=q.float()), dict(q=q[:, :, :32]), dict(q=q[:, ::2]), dict(q=q[:1].expand(4, 4, 64)), dict(q=q[:3]),
+           dict(table=table.long()), dict(table=table[:1]), dict(table=table[:, :0]), dict(lens=lens.long()), dict(lens=lens[:1]),
+           dict(table=table.t().contiguous().t()), dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")),
+           dict(gate=q[:2]), dict(gate=q.float()), dict(out=torch.empty(4, 256, device=dev)),
+           dict(out=torch.empty(4, 512, device=dev, dtype=BF16)[:, :256])]
+    for change in bad:
+        kw = dict(q=q, table=table, lens=lens)
+        kw.update(change)
+        a = (kw.pop("q"), cache, kw.pop("table"), kw.pop("lens"))
+        with pytest.raises(ValueError):
+            paged.attention(*a, **kw)
+        if "q" not in change or change["q"].shape[0] != 3:
+            with pytest.raises(ValueError):
+                paged.prompt_attention(*a, cu, **kw)
+    with pytest.raises(NotImplementedError):
+        paged.attention(q.repeat(5, 1, 1)[:18], cache, table, lens)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        paged.attention(q.cpu(), cache, table, lens)
+    for c in (cu.long(), cu[:2]):
+        with pytest.raises(ValueError):
+            paged.prompt_attention(q, cache, table, lens, c)
+    qkv = torch.zeros((4, 8 * 64), device=dev, dtype=BF16)
+    w = torch.ones(64, device=dev, dtype=BF16)
+    cos = torch.ones(80, 8, device=dev)
+    for change in (dict(qkv=qkv[:, :500]), dict(qkv=qkv.float()), dict(qkv=qkv[:1].expand(4, 512)), dict(n_heads=0), dict(n_heads=5),
+                   dict(gated=True), dict(q_norm=w[:32]), dict(k_norm=w.float()), dict(cos=cos), dict(cos=cos, sin=cos[:9]),
+                   dict(cos=cos.double(), sin=cos.double()), dict(eps=-1.0), dict(cu=cu.long()), dict(qkv=qkv[:3])):
+        kw = dict(qkv=qkv, n_heads=4)
+        kw.update(change)
+        with pytest.raises(ValueError):
+            paged.append_qkv(kw.pop("qkv"), cache, table, lens, kw.pop("cu", None), **kw)
+    with pytest.raises(NotImplementedError):
+        paged.append_qkv(qkv, cache, table, lens, n_heads=4, cos=torch.ones(80, 12, device=dev), sin=torch.ones(80, 12, device=dev))
+    empty = paged.append_qkv(qkv[:0], cache, table, lens, n_heads=4)[0]
+    assert empty.shape == (0, 4, 64)
+    assert paged.attention(q[:0], cache, table, lens).shape == paged.prompt_attention(q[:0], cache, table, lens, cu).shape == (0, 256)
+    k = torch.zeros((4, 2, 16, 64), device=dev, dtype=BF16)
+    for kk, vv in ((k, k[:3]), (k.float(), k.float()), (k[:, :, ::2], k[:, :, ::2]), (k[0], k[0])):
+        with pytest.raises(ValueError):
+            paged.PagedCache(kk, vv)
+    no_error()
