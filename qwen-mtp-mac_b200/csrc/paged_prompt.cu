@@ -424,12 +424,14 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         };
         bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
         ++work;
-        for (int w = 0; w < ts.chains; ++w) scores(w, 0, w == ts.chains - 1);
-        for (int j = 0; j < subs; ++j) {
-          if (j + 1 < subs)
-            for (int w = 0; w < ts.chains; ++w) scores(w, j + 1, w == ts.chains - 1);
-          for (int w = 0; w < ts.chains; ++w) values(w, j, w == ts.chains - 1);
-        }
+        // per row tile S0 S1 | O0 S2 | O1 S3 ...: the next scores are always under way while the softmax works
+        for (int j = 0; j < min(2, subs); ++j)
+          for (int w = 0; w < ts.chains; ++w) scores(w, j, w == ts.chains - 1);
+        for (int j = 0; j < subs; ++j)
+          for (int w = 0; w < ts.chains; ++w) {
+            values(w, j, w == ts.chains - 1);
+            if (j + 2 < subs) scores(w, j + 2, w == ts.chains - 1);
+          }
         e0 += 2 * nt * E;
         for (int w = 0; w < ts.chains; ++w) { g[w] += subs; ++finished[w]; }
       }
