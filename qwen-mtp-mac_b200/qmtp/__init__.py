@@ -8,6 +8,7 @@ Modules mirror the reference's Python surface (aulafy/qwen-mtp-mac):
   mtp          MTP decoder: greedy or sampled verify, prefix cache     <- mtp.py, engine.py
   loader       safetensors / Ollama checkpoints -> decoder weights     <- qwen_ollama.py, mtp.py:61-70
   moe, moe_ep  MXFP4 / NVFP4 expert decode, expert parallelism         <- experiments/deepseek_moe
+  paged        attention of several sequences over a paged cache       (no counterpart)
 and are backed by libqmtp.so (C ABI in include/qmtp.h, kernels in csrc/).
 """
 __version__ = "0.1.0"
