@@ -1,17 +1,24 @@
 // Prompt attention over the paged cache on the tensor cores (tcgen05), for a ragged batch of chunks.
 //
-// A CTA per SM takes items of work in turn: NQ tiles of 128 query rows (128 / G tokens x the G query heads of a
-// key head: all of them read the same keys).  It walks the key tiles (128 keys) they see with the running maximum m and sum l of the
-// softmax.  Per key tile: S = Q K^T into TMEM; the tile's 128 threads, one row each, turn S into weights
-// P = 2^(S scale2 - m) in place (bf16); O += P V with P from TMEM.  O stays in TMEM and is rescaled only
-// when a row's maximum has grown by more than 2^kSlack since the last rescale, which leaves P <= 2^kSlack;
-// the final division by l takes it out again.
+// Work comes in items: two tiles of 128 query rows (128 / G tokens x the G query heads of a key head, which all read
+// the same keys) and the key tiles (128 keys) that they see, walked with the running maximum m and sum l of the softmax.
+// Per score tile: S = Q K^T into TMEM; the row tile's 128 threads, one row each, turn S into weights
+// P = 2^(S scale2 - m) in place (bf16); O += P V with P from TMEM.  O stays in TMEM and is rescaled only when a
+// row's maximum has grown by more than 2^kSlack since the last rescale, which leaves P <= 2^kSlack; the final division
+// by l takes it out again.
 //   warps 0 .. 4 NQ - 1   softmax, and at the end O / l, the gate and the store
 //   warp 4 NQ             which item is next; TMA: pages into a ring of tiles (128-byte swizzle)
-//   warp 4 NQ + 1         MMA issue
-// Each row tile has two score tiles in TMEM: the scores of the next keys run under this one's softmax.  Dh 256: one
-// row tile, 128 keys a score tile.  Dh 128, 64: two row tiles, 64 keys a score tile, where the tensor core and
-// the exponentials take about as long as each other.  TMEM: O in columns [0, 256), S in [256, 512).
+//   warp 4 NQ + 1         MMA issue, by one thread
+// Each row tile has two score tiles in TMEM: the scores of the next keys run under this one's softmax.  TMEM: O in
+// columns [0, 256), S in [256, 512).
+//
+// Dh 256: a pair of CTAs, a row tile each, 128 keys a score tile.  The tensor core takes 2048 cycles a key tile, the
+// softmax 1850; 128 rows against 128 KB of keys and values would need 64 bytes a cycle of every SM, what L2 has.  So the
+// pair shares each tile (cta_group::2: half of K's keys and of V's dims in each CTA), half the traffic and twice the ring.
+// 16384 tokens, 16 / 4 heads of 256, causal: 1361 us, 1.62 PFLOP/s, 2166 cycles a key tile; by single CTAs 1600 us.
+// Dh 128, 64: one CTA, both row tiles, 64 keys a score tile.  Here the exponentials (16 a cycle and SM) take as long as
+// the products, and two warps a scheduler do not hide all of each other's latencies: 6000 tokens, 32 / 8 heads of 128:
+// 287 us, 1.03 PFLOP/s.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -24,9 +31,10 @@ constexpr float kSlack = 8.0f;
 
 template <int Dh>
 struct PromptCfg {
-  static constexpr int NQ = Dh == 256 ? 1 : 2;               // row tiles per CTA
-  static constexpr int E = Dh == 256 ? 2 : 1;                // ring entries per K or V tile (halves of 32 KB)
-  static constexpr int entry = kKeys * Dh * 2 / E;           // bytes
+  static constexpr bool PAIR = Dh == 256;                    // a pair of CTAs works on an item
+  static constexpr int NQ = PAIR ? 1 : 2;                    // row tiles per CTA
+  static constexpr int entry = kKeys * Dh * 2 * NQ / 2;      // bytes of a ring entry: a K or V tile, or the CTA's half
+  static constexpr int box = kKeys * NQ / 2;                 // most rows of a copy
   static constexpr int SUB = kKeys / NQ;                     // keys of a score tile (two per row tile in TMEM)
   static constexpr int stages = Dh == 64 ? 8 : 5;
   static constexpr int threads = NQ * 128 + 64;
@@ -53,11 +61,14 @@ struct PromptItem {
   int b, kh, split, tok0, n, c0, len;  // b < 0: no more work
 };
 
+// PAIR: full, p_full, q_full and item_empty are used in the first CTA, where the MMAs are issued, by both CTAs' warps; the
+// others tell each CTA of what happened.
 struct PromptBars {
   uint64_t full[8], empty[8], q_full, q_empty, s_full[2][2], p_full[2][2][2];  // [row tile][score tile][64 keys]
   uint64_t pv[2];    // a phase per score tile but an item's last: O holds the products up to it
   uint64_t done[2];  // an item's last product
   uint64_t item_full[2], item_empty[2], next_full;
+  uint64_t tail;     // PAIR: this CTA's half of a V tile in which the sequence ends
   alignas(16) uint4 next[1];
   PromptItem item[2];
   uint32_t tmem;
@@ -71,7 +82,7 @@ struct PromptTiles {
   __device__ __forceinline__ PromptTiles(const PromptItem& x, const PromptArgs& a, int NQ) {
     const int SUB = kKeys / NQ;
     p_first = x.len - x.n + x.tok0;
-    p_last = x.len - x.n + min(x.n, x.tok0 + NQ * a.tpt) - 1;
+    p_last = x.len - x.n + min(x.n, x.tok0 + 2 * a.tpt) - 1;
     chains = NQ == 1 || x.tok0 + a.tpt >= x.n ? 1 : 2;  // row tiles that hold a token
     // key tiles: [0, sink_tiles), then [lo / 128, p_last / 128]
     lo = a.vis.first(max(p_first, 0));
@@ -182,6 +193,73 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
     }
   }
 }
+// ---- a pair of CTAs (cta_group::2): the MMAs of both are issued by the first; each holds its 128 rows of Q, S, P and O,
+// and half of every K tile (64 keys) and V tile (128 dims), which the tensor cores of both read.
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+__device__ __forceinline__ uint32_t in_cta(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same without the release of this thread's memory operations (a release at cluster scope takes about 1000 cycles
+// here): for tensor memory, whose order the tcgen05 fences on both sides give.
+__device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// warp_wait / bar_wait for what another CTA of the cluster released.
+__device__ __forceinline__ bool bar_wait_cluster(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
+  const bool ok = bar_wait(dead, bar, parity, err);
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  return ok;
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, int x, int y, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const void* tmap, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (!PAIR) return umma_bf16(d, a, b, idesc, accumulate);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (!PAIR) return umma_bf16_ts(d, a, b, idesc, accumulate);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier, PAIR: in both CTAs, when the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  if (!PAIR) return umma_commit(bar);
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(uint16_t(3))
+      : "memory");
+}
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t x;
@@ -193,7 +271,8 @@ __global__ void __launch_bounds__(PromptCfg<Dh>::threads, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, PagedView c, PromptArgs a) {
   using Cfg = PromptCfg<Dh>;
-  constexpr int NQ = Cfg::NQ, E = Cfg::E, NS = Cfg::stages, SUB = Cfg::SUB, CB = Dh / 64;  // CB: 64-dim column blocks
+  constexpr bool PAIR = Cfg::PAIR;
+  constexpr int NQ = Cfg::NQ, NS = Cfg::stages, SUB = Cfg::SUB, CB = Dh / 64;  // CB: 64-dim column blocks
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -202,7 +281,16 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   PromptBars* bars = reinterpret_cast<PromptBars*>(s_ring + NS * Cfg::entry);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
-  if (warp == 4 * NQ + 1) tmem_alloc(&bars->tmem, 512);
+  const int rank = PAIR ? int(cluster_rank()) : 0;
+
+  if (warp == 4 * NQ + 1) {
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bars->tmem)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(&bars->tmem, 512);
+    }
+  }
   if (warp == 4 * NQ && lane == 0) {
     prefetch_tensormap(&tq);
     prefetch_tensormap(&tk);
@@ -211,16 +299,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     mbar_init(&bars->q_full, 1);
     mbar_init(&bars->q_empty, 1);
     mbar_init(&bars->next_full, 1);
+    mbar_init(&bars->tail, 1);
     for (int i = 0; i < 2; ++i) {
       for (int k = 0; k < 2; ++k) {
         mbar_init(&bars->s_full[i][k], 1);
-        mbar_init(&bars->p_full[i][k][0], 128);
-        mbar_init(&bars->p_full[i][k][1], 128);
+        mbar_init(&bars->p_full[i][k][0], PAIR ? 8 : 128);
+        mbar_init(&bars->p_full[i][k][1], PAIR ? 8 : 128);
       }
       mbar_init(&bars->pv[i], 1);
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->item_full[i], 1);
-      mbar_init(&bars->item_empty[i], 4 * NQ + 1);
+      mbar_init(&bars->item_empty[i], PAIR ? 10 : 4 * NQ + 1);
     }
     bars->dead = 0;
     fence_mbar_init();
@@ -228,6 +317,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   pdl_wait();
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();  // the barriers of both CTAs are ready
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   // ring position, within an item, of K(t), V(t): Dh 256 loads K0 K1 V0 K2 V1 ..., otherwise K0 V0 K1 V1 ...
@@ -236,16 +326,16 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
 
   if (warp == 4 * NQ) {
     // -------------------------------------------------------------------- items and TMA
-    const int TT = NQ * a.tpt;                                             // tokens per item
-    const int box = min(1 << c.page_log, kKeys / E), parts = kKeys / box;  // rows per box, boxes down a tile
+    const int TT = 2 * a.tpt;                                             // tokens per item
+    const int box = min(1 << c.page_log, Cfg::box), parts = kKeys / box;  // rows per box, boxes down a tile
     const long long none = (c.pages * c.nkv) << c.page_log;                // past the end: reads as zeros
     int seq = 0, before = 0;  // sequences [0, seq) hold `before` row tiles: items come in rising order
-    int e0 = 0, issued = 0, loads = 0;
-    long long u = blockIdx.x;
+    int e0 = 0, issued = 0, loads = 0, tails = 0;
+    long long u = blockIdx.x / (PAIR ? 2 : 1);
     for (int i = 0;; ++i) {
       // The next item: that of a block of the grid that has not started, taken over while this one runs.  With no more
       // blocks than SMs each finds a place of its own, and none is taken.
-      if (lane == 0 && a.takes_over) {
+      if (lane == 0 && rank == 0 && a.takes_over) {
         mbar_expect_tx(&bars->next_full, 16);
         next_block_request(bars->next, &bars->next_full);
       }
@@ -254,7 +344,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       x.split = int(u % a.splits);
       x.kh = int(u / a.splits % c.nkv);
       const long long tile = u / a.splits / c.nkv;
-      while (seq < c.B) {
+      while ((rank == 0 || i == 0) && seq < c.B) {
         const int k = seq + lane;
         int n = 0, c0 = 0, len = 0;
         if (k < c.B) {
@@ -293,11 +383,27 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         if (lane == 0) {
           bars->item[at & 1] = y;
           mbar_arrive(&bars->item_full[at & 1]);
+          if (PAIR && rank == 0 && at > 0) {
+            const uint32_t to = in_cta(&bars->item[at & 1], 1);
+            const int v[7] = {y.b, y.kh, y.split, y.tok0, y.n, y.c0, y.len};
+#pragma unroll
+            for (int k = 0; k < 7; ++k) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + 4 * k), "r"(v[k]) : "memory");
+            arrive_cluster(in_cta(&bars->item_full[at & 1], 1));
+          }
         }
         __syncwarp();
         return ok;
       };
-      const bool ok = hand_out(x, i);
+      bool ok;
+      if (rank == 0 || i == 0) {
+        ok = hand_out(x, i);
+      } else {  // the second CTA finds the first item itself and is told of the others
+        ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(&bars->dead, &bars->item_full[i & 1], (i >> 1) & 1, a.err));
+        if (!ok) break;
+        x = bars->item[i & 1];
+        __syncwarp();
+      }
+      if (rank == 1 && lane == 0) arrive_cluster(in_first_cta(&bars->item_empty[i & 1]));
       const PromptTiles ts(x, a, NQ);
       if (ok && x.b >= 0 && ts.nt > 0) {
         // cache row of part `lane` of the tile at key j (a page that no row needs is not looked at)
@@ -308,49 +414,67 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           const long long r = cache_row(c, x.b, x.kh, key, a.err);
           return int(r < 0 ? none : r);
         };
-        auto load = [&](const CUtensorMap* map, int pos, bool is_v, int row) {
-#pragma unroll
-          for (int h = 0; h < E; ++h) {
-            const int e = e0 + pos * E + h, st = e % NS;
-            if (!warp_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err)) return;
-            if (lane == 0) mbar_expect_tx(&bars->full[st], Cfg::entry);
-            __syncwarp();
-            issued = e + 1;
-            uint8_t* dst = s_ring + st * Cfg::entry;
-            // an entry: K all keys x half the dims, V half the keys x all dims (E == 2), else the whole tile
-            const int ncb = is_v ? CB : CB / E, np = is_v ? parts / E : parts, rows = is_v ? kKeys / E : kKeys;
-            const int part = lane / ncb, cb = lane - part * ncb;
-            const int r = __shfl_sync(0xFFFFFFFFu, row, (is_v ? h * np : 0) + min(part, np - 1));
-            if (part < np)
-              tma_load_2d(dst + cb * rows * 128 + part * box * 128, map, (is_v ? cb : h * ncb + cb) * 64, r, &bars->full[st],
-                          policy_evict_last());
+        auto load = [&](const CUtensorMap* map, int pos, bool is_v, int row, bool tail) {
+          const int e = e0 + pos, st = e % NS;
+          if (!warp_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err)) return;
+          // PAIR: the copies of both CTAs count on the first one's barrier; those of a V tile in which the sequence ends
+          // on their own CTA's, whose softmax warps clear it and answer with their weights
+          if (lane == 0) {
+            if (PAIR && tail) mbar_expect_tx(&bars->tail, Cfg::entry);
+            if (PAIR && tail && rank == 0) mbar_arrive(&bars->full[st]);
+            if (!(PAIR && tail) && rank == 0) mbar_expect_tx(&bars->full[st], Cfg::entry * (PAIR ? 2 : 1));
           }
+          __syncwarp();
+          issued = e + 1;
+          uint8_t* dst = s_ring + st * Cfg::entry;
+          // an entry: a tile, or for a pair 64 of K's keys with all dims, all of V's keys with 128 dims
+          const int ncb = PAIR && is_v ? CB / 2 : CB, np = PAIR && !is_v ? parts / 2 : parts, rows = PAIR && !is_v ? kKeys / 2 : kKeys;
+          const int part = lane / ncb, cb = lane - part * ncb;
+          const int r = __shfl_sync(0xFFFFFFFFu, row, (PAIR && !is_v ? rank * np : 0) + min(part, np - 1));
+          if (part < np) {
+            uint8_t* to = dst + cb * rows * 128 + part * box * 128;
+            const int col = (PAIR && is_v ? rank * ncb + cb : cb) * 64;
+            if (PAIR && !tail)
+              tma_load_2d_pair(to, map, col, r, in_first_cta(&bars->full[st]), policy_evict_last());
+            else
+              tma_load_2d(to, map, col, r, PAIR ? &bars->tail : &bars->full[st], policy_evict_last());
+          }
+          if (tail) ++tails;
         };
         auto load_q = [&] {
           if (!warp_wait(&bars->dead, &bars->q_empty, (loads & 1) ^ 1, a.err)) return;
-          if (lane == 0) mbar_expect_tx(&bars->q_full, uint32_t(ts.chains) * a.G * a.tpt * Dh * 2);
+          if (lane == 0 && rank == 0) mbar_expect_tx(&bars->q_full, uint32_t(PAIR ? 2 : ts.chains) * a.G * a.tpt * Dh * 2);
           __syncwarp();
           if (lane < ts.chains * CB) {
             const int w = lane / CB, cb = lane - w * CB;
-            tma_load_3d(s_q + w * Cfg::q_bytes + cb * kRows * 128, &tq, cb * 64, x.kh * a.G, x.c0 + x.tok0 + w * a.tpt,
-                        &bars->q_full);
+            uint8_t* to = s_q + w * Cfg::q_bytes + cb * kRows * 128;
+            const int z = x.c0 + x.tok0 + (PAIR ? rank : w) * a.tpt;
+            if (PAIR)
+              tma_load_3d_pair(to, &tq, cb * 64, x.kh * a.G, z, in_first_cta(&bars->q_full));
+            else
+              tma_load_3d(to, &tq, cb * 64, x.kh * a.G, z, &bars->q_full);
           }
           ++loads;
         };
+        auto ends = [&](int t) { return ts.key(t) + kKeys > x.len; };
         const bool first = loads == 0;
         if (first) load_q();  // later its place is still in use: behind the first keys
         int row = part_row(ts.key(0)), row_next = ts.nt > 1 ? part_row(ts.key(1)) : 0;
-        load(&tk, pos_k(0), false, row);
+        load(&tk, pos_k(0), false, row, false);
         if (!first) load_q();
         for (int t = 0; t < ts.nt; ++t) {
           const int row_after = t + 2 < ts.nt ? part_row(ts.key(t + 2)) : 0;
-          if (NQ == 2) load(&tv, pos_v(t, ts.nt), true, row);
-          if (t + 1 < ts.nt) load(&tk, pos_k(t + 1), false, row_next);
-          if (NQ == 1) load(&tv, pos_v(t, ts.nt), true, row);
+          if (NQ == 2) load(&tv, pos_v(t, ts.nt), true, row, false);
+          if (t + 1 < ts.nt) load(&tk, pos_k(t + 1), false, row_next, false);
+          if (NQ == 1) load(&tv, pos_v(t, ts.nt), true, row, ends(t));
           row = row_next;
           row_next = row_after;
         }
-        e0 += 2 * ts.nt * E;
+        e0 += 2 * ts.nt;
+      }
+      if (rank == 1) {
+        if (x.b < 0) break;
+        continue;
       }
       int next = -1;
       if (a.takes_over && bar_wait(&bars->dead, &bars->next_full, i & 1, a.err)) next = next_block(bars->next);
@@ -361,18 +485,19 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         hand_out(x, i + 1);
         break;
       }
-      u = next;
+      u = next / (PAIR ? 2 : 1);
     }
     if (*reinterpret_cast<volatile int*>(&bars->dead)) {  // copies in flight end before the CTA does
-      if (loads > 0) mbar_wait_bounded(&bars->q_full, (loads - 1) & 1, a.err, 1u << 22);
-      for (int e = max(0, issued - NS); e < issued; ++e)
+      if (tails > 0) mbar_wait_bounded(&bars->tail, (tails - 1) & 1, a.err, 1u << 22);
+      if (loads > 0 && rank == 0) mbar_wait_bounded(&bars->q_full, (loads - 1) & 1, a.err, 1u << 22);
+      for (int e = rank ? issued : max(0, issued - NS); e < issued; ++e)
         mbar_wait_bounded(&bars->full[e % NS], (e / NS) & 1, a.err, 1u << 22);
     }
   } else if (warp == 4 * NQ + 1) {
     // -------------------------------------------------------------------- MMA
-    if (elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16(kRows, Cfg::SUB);
-      constexpr uint32_t idesc_o = umma_idesc_bf16(kRows, Dh) | (1u << 16);  // B (V) is MN-major
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc_s = umma_idesc_bf16(PAIR ? 2 * kRows : kRows, Cfg::SUB);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(PAIR ? 2 * kRows : kRows, Dh) | (1u << 16);  // B (V) is MN-major
       int e0 = 0, items = 0, work = 0;
       int g[2] = {0, 0};  // score tiles so far, per row tile
       int finished[2] = {0, 0};
@@ -387,40 +512,35 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const int subs = ts.subs;
         auto scores = [&](int w, int j, bool last) {  // S = Q_w K^T of score tile j
           const int buf = (g[w] + j) & 1, t = j / NQ, r0 = (j - t * NQ) * Cfg::SUB;
+          const int e = e0 + pos_k(t), st = e % NS;
+          bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+          tc_fence_after();
+          const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes), 16, 1024);
+          const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, 16, 1024);
 #pragma unroll
-          for (int h = 0; h < E; ++h) {
-            const int e = e0 + pos_k(t) * E + h, st = e % NS;
-            bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
-            tc_fence_after();
-            const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes) + h * (CB / E) * kRows * 128, 16, 1024);
-            const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, 16, 1024);
-#pragma unroll
-            for (int k = 0; k < Dh / E / 16; ++k) {
-              const uint32_t off = ((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4;
-              umma_bf16(tmem + 256 + (2 * w + buf) * Cfg::SUB, qd + off, kd + off, idesc_s, (h | k) != 0);
-            }
-            if (last && (j % NQ == NQ - 1 || j + 1 == subs)) umma_commit(&bars->empty[st]);
-            if (last && j + 1 == subs && h + 1 == E) umma_commit(&bars->q_empty);
-          }
-          umma_commit(&bars->s_full[w][buf]);
+          for (int k = 0; k < Dh / 16; ++k)
+            mma_ss<PAIR>(tmem + 256 + (2 * w + buf) * Cfg::SUB, qd + (((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4),
+                         kd + (((k >> 2) * (PAIR ? kKeys / 2 : kKeys) * 128 + (k & 3) * 32) >> 4), idesc_s, k != 0);
+          if (last && (j % NQ == NQ - 1 || j + 1 == subs)) mma_commit<PAIR>(&bars->empty[st]);
+          if (last && j + 1 == subs) mma_commit<PAIR>(&bars->q_empty);
+          mma_commit<PAIR>(&bars->s_full[w][buf]);
         };
         auto values = [&](int w, int j, bool last) {  // O_w += P V of score tile j
           const int buf = (g[w] + j) & 1, parity = ((g[w] + j) >> 1) & 1, t = j / NQ, r0 = (j - t * NQ) * Cfg::SUB;
+          const int e = e0 + pos_v(t, nt), st = e % NS;
+          bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
 #pragma unroll
           for (int hf = 0; hf < Cfg::SUB / 64; ++hf) {  // 64 keys, as the softmax hands them over
-            constexpr int rows = kKeys / E;
-            const int e = e0 + pos_v(t, nt) * E + hf, st = e % NS;
-            bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
             bar_wait(&bars->dead, &bars->p_full[w][buf][hf], parity, a.err);
             tc_fence_after();
-            const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, rows * 128, 1024);
+            const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + (r0 + hf * 64) * 128, kKeys * 128, 1024);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_bf16_ts(tmem + w * Dh, tmem + 256 + (2 * w + buf) * Cfg::SUB + hf * 32 + k * 8, vd + k * (2048 >> 4),
+              mma_ts<PAIR>(tmem + w * Dh, tmem + 256 + (2 * w + buf) * Cfg::SUB + hf * 32 + k * 8, vd + k * (2048 >> 4),
                            idesc_o, j > 0 || (hf | k) != 0);
-            if (last && (j % NQ == NQ - 1 || j + 1 == subs)) umma_commit(&bars->empty[st]);
           }
-          umma_commit(j + 1 < subs ? &bars->pv[w] : &bars->done[w]);
+          if (last && (j % NQ == NQ - 1 || j + 1 == subs)) mma_commit<PAIR>(&bars->empty[st]);
+          mma_commit<PAIR>(j + 1 < subs ? &bars->pv[w] : &bars->done[w]);
         };
         bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
         ++work;
@@ -432,7 +552,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             values(w, j, w == ts.chains - 1);
             if (j + 2 < subs) scores(w, j + 2, w == ts.chains - 1);
           }
-        e0 += 2 * nt * E;
+        e0 += 2 * nt;
         for (int w = 0; w < ts.chains; ++w) { g[w] += subs; ++finished[w]; }
       }
       // every product is over before the tensor memory is given back
@@ -446,21 +566,29 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     const uint32_t lane_base = uint32_t(warp & 3) << 21;  // TMEM lane 32 (warp % 4) in bits 16..
     const uint32_t t_o = tmem + lane_base + w * Dh;
     int g = 0, pvs = 0, finished = 0;  // score tiles, phases of pv and of done so far
-    int e0 = 0;                        // ring entries of the items so far
+    int e0 = 0, tails = 0;             // ring entries of the items so far, V tiles cleared
     for (int items = 0;; ++items) {
-      if (!warp_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)) break;
+      if (!__all_sync(0xFFFFFFFFu, PAIR ? bar_wait_cluster(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)
+                                        : bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)))
+        break;
       const PromptItem x = bars->item[items & 1];
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->item_empty[items & 1]);
+      if (lane == 0) {
+        if (PAIR)
+          arrive_cluster(in_first_cta(&bars->item_empty[items & 1]));
+        else
+          mbar_arrive(&bars->item_empty[items & 1]);
+      }
       if (x.b < 0) break;
       const PromptTiles ts(x, a, NQ);
       const int e_item = e0;
-      e0 += 2 * ts.nt * E;
+      e0 += 2 * ts.nt;
       if (w >= ts.chains) continue;
-      const int nt = ts.nt, i_tok = x.tok0 + w * a.tpt + r / a.G;  // token of the chunk
+      const int tile0 = x.tok0 + (PAIR ? rank : w) * a.tpt;    // the row tile's first token of the chunk
+      const int nt = ts.nt, i_tok = tile0 + r / a.G;
       const bool valid = r < a.G * a.tpt && i_tok < x.n;
       const int h = x.kh * a.G + r % a.G, p = x.len - x.n + i_tok;
-      const int pw0 = x.len - x.n + x.tok0 + w * a.tpt, pw1 = min(x.len - 1, pw0 + a.tpt - 1);  // the row tile's positions
+      const int pw0 = x.len - x.n + tile0, pw1 = min(x.len - 1, pw0 + a.tpt - 1);  // the row tile's positions
       float m = -INFINITY, l = 0.0f;  // m: maximum in use, in units of scale2
       for (int j = 0; j < ts.subs; ++j) {
         const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, j0 = ts.key(t) + r0;
@@ -473,19 +601,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         if (j0 + SUB > x.len) {
           // The sequence ends in this tile: the values behind its end may be anything, and their weight 0 has to stay
           // 0.  They are cleared before the weights are handed over.
-#pragma unroll
-          for (int k = 0; k < E; ++k) {
-            constexpr int rows = SUB / E;
-            const int e = e_item + pos_v(t, nt) * E + k, st = e % NS;
-            warp_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
-            for (int i = r; i < CB * rows * 8; i += 128) {
-              const int row = (i >> 3) % rows, cb = (i >> 3) / rows;
-              if (j0 + k * rows + row >= x.len)
-                *reinterpret_cast<uint4*>(s_ring + st * Cfg::entry + ((cb * (kKeys / E) + r0 + row) * 8 + (i & 7)) * 16) =
-                    make_uint4(0, 0, 0, 0);
-            }
+          const int e = e_item + pos_v(t, nt), st = e % NS;
+          warp_wait(&bars->dead, PAIR ? &bars->tail : &bars->full[st], PAIR ? tails & 1 : (e / NS) & 1, a.err);
+          ++tails;
+          for (int i = r; i < Cfg::entry / 16 / kKeys * SUB; i += 128) {
+            const int row = (i >> 3) % SUB, cb = (i >> 3) / SUB;
+            if (j0 + row >= x.len)
+              *reinterpret_cast<uint4*>(s_ring + st * Cfg::entry + ((cb * kKeys + r0 + row) * 8 + (i & 7)) * 16) =
+                  make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async();
+          if (PAIR) asm volatile("fence.acq_rel.cluster;" ::: "memory");
           __syncwarp();
         }
 #pragma unroll
@@ -540,7 +666,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (c & 1) {  // 64 keys are handed over as soon as they are stored
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&bars->p_full[w][buf][c >> 1]);
+            if (PAIR) {
+              __syncwarp();
+              if (lane == 0) arrive_cluster_relaxed(in_first_cta(&bars->p_full[w][buf][c >> 1]));
+            } else {
+              mbar_arrive(&bars->p_full[w][buf][c >> 1]);
+            }
           }
         }
         float x, y;
@@ -634,7 +765,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       while (todo) {
         const int src = __ffs(todo) - 1;
         todo &= todo - 1;
-        const int rr = (tid & 127 & ~31) + src, ti = x.tok0 + w * a.tpt + rr / a.G, hh = x.kh * a.G + rr % a.G;
+        const int rr = (tid & 127 & ~31) + src, ti = tile0 + rr / a.G, hh = x.kh * a.G + rr % a.G;
         const long long tr = x.c0 + ti;
         float mm = -INFINITY, ll = 0.0f, oo[Dh / 32] = {};
         for (int t = 0; t < nt; ++t)
@@ -658,8 +789,14 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();  // neither CTA's memory is used by the other any more
   tc_fence_after();
-  if (warp == 4 * NQ + 1) tmem_dealloc(tmem, 512);
+  if (warp == 4 * NQ + 1) {
+    if (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    else
+      tmem_dealloc(tmem, 512);
+  }
 }
 
 // Joins the splits of a row: one warp per (row, head), splits in order.  A row of no sequence is left alone.
@@ -701,14 +838,14 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedView c, PromptArg
 // ----------------------------------------------------------------------------- host
 // Items of work that a call has at most (the sequences' row counts are only known on the device).
 static long long prompt_items(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
-  const int NQ = c->Dh == 256 ? 1 : 2, TT = NQ * (kRows / (a->n_q / c->n_kv));
+  const int TT = 2 * (kRows / (a->n_q / c->n_kv));
   return ((long long)a->T / TT + std::min(a->T, c->B)) * c->n_kv;
 }
 
 // With fewer items than SMs the key tiles of each are split, down to four tiles a split: two (512 tokens of 16 / 4
 // heads of 256 in 128 CTAs) measured 25.1 us, whole items (64 CTAs) 18.1; 128 tokens behind 8000 want the split, 38 for 117 us.
 static int prompt_splits(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
-  const long long items = prompt_items(a, c), sms = sm_count();
+  const long long items = prompt_items(a, c), sms = c->Dh == 256 ? sm_count() / 2 : sm_count();
   long long tiles = ((long long)c->table_w * c->page + kKeys - 1) / kKeys;
   if (a->window > 0) tiles = std::min(tiles, ((long long)a->window + kRows) / kKeys + 2 + a->sinks / kKeys);
   return int(std::max<long long>(1, std::min({sms / items, tiles / 4, 32ll})));
@@ -727,11 +864,13 @@ static int launch_prompt(const qmtp_paged_args* args, const PagedView& v, Prompt
   const cuuint64_t qd[3] = {Dh, cuuint64_t(a.nq), cuuint64_t(a.T)}, qs[2] = {Dh * 2, cuuint64_t(a.q_ld) * 2};
   const cuuint32_t qb[3] = {64, cuuint32_t(a.G), cuuint32_t(a.tpt)};
   const cuuint64_t kd[2] = {Dh, cuuint64_t((v.pages * v.nkv) << v.page_log)}, ks[1] = {Dh * 2};
-  const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, kKeys / Cfg::E))};
+  const cuuint32_t kb[2] = {64, cuuint32_t(std::min(1 << v.page_log, Cfg::box))};
   if (!encode_pages(&tq, a.q, 3, qd, qs, qb) || !encode_pages(&tk, v.k, 2, kd, ks, kb) || !encode_pages(&tv, v.v, 2, kd, ks, kb))
     return QMTP_ERR_CUDA;
-  a.takes_over = items * a.splits > sm_count();
-  launch_kernel(paged_prompt_kernel<Dh>, dim3(unsigned(items * a.splits)), dim3(Cfg::threads), Cfg::smem, st, tq, tk, tv, v, a);
+  constexpr int per = Cfg::PAIR ? 2 : 1;  // CTAs of an item
+  a.takes_over = items * a.splits * per > sm_count();
+  launch_kernel_cluster(paged_prompt_kernel<Dh>, dim3(unsigned(items * a.splits * per)), dim3(Cfg::threads), Cfg::smem, st, per,
+                        tq, tk, tv, v, a);
   if (a.splits > 1)
     launch_kernel(prompt_join_kernel<Dh>, dim3(unsigned(((long long)a.T * a.nq + 7) / 8)), dim3(256), 0, st, v, a);
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
