@@ -8,7 +8,7 @@
 // by l takes it out again.
 //   warps 0 .. 4 NQ - 1   softmax, and at the end O / l, the gate and the store
 //   warp 4 NQ             which item is next; TMA: pages into a ring of tiles (128-byte swizzle)
-//   warp 4 NQ + 1         MMA issue, by one thread
+//   warps 4 NQ + 1 ..     MMA issue, by a thread for each row tile
 // Each row tile has two score tiles in TMEM: the scores of the next keys run under this one's softmax.  TMEM: O in
 // columns [0, 256), S in [256, 512).
 //
@@ -37,7 +37,7 @@ struct PromptCfg {
   static constexpr int box = kKeys * NQ / 2;                 // most rows of a copy
   static constexpr int SUB = kKeys / NQ;                     // keys of a score tile (two per row tile in TMEM)
   static constexpr int stages = Dh == 64 ? 8 : 5;
-  static constexpr int threads = NQ * 128 + 64;
+  static constexpr int threads = NQ * 128 + 32 + NQ * 32;
   static constexpr int q_bytes = kRows * Dh * 2;
   static constexpr int smem = NQ * q_bytes + stages * entry + 1024 + 512;
 };
@@ -193,6 +193,14 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
     }
   }
 }
+// Two row tiles: the warps of both that share a scheduler take turns at the exponentials.  Side by side they fall into
+// step, share the exponential unit and then leave it idle together while they wait and search maxima.
+__device__ __forceinline__ void turn_wait(int w, int quarter) {
+  asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(1 + 2 * quarter + w) : "memory");
+}
+__device__ __forceinline__ void turn_pass(int w, int quarter) {
+  asm volatile("barrier.cta.arrive.aligned %0, 64;" ::"r"(1 + 2 * quarter + (w ^ 1)) : "memory");
+}
 // ---- a pair of CTAs (cta_group::2): the MMAs of both are issued by the first; each holds its 128 rows of Q, S, P and O,
 // and half of every K tile (64 keys) and V tile (128 dims), which the tensor cores of both read.
 __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
@@ -295,9 +303,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     prefetch_tensormap(&tq);
     prefetch_tensormap(&tk);
     prefetch_tensormap(&tv);
-    for (int i = 0; i < NS; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
+    for (int i = 0; i < NS; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], NQ); }
     mbar_init(&bars->q_full, 1);
-    mbar_init(&bars->q_empty, 1);
+    mbar_init(&bars->q_empty, NQ);
     mbar_init(&bars->next_full, 1);
     mbar_init(&bars->tail, 1);
     for (int i = 0; i < 2; ++i) {
@@ -309,7 +317,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       mbar_init(&bars->pv[i], 1);
       mbar_init(&bars->done[i], 1);
       mbar_init(&bars->item_full[i], 1);
-      mbar_init(&bars->item_empty[i], PAIR ? 10 : 4 * NQ + 1);
+      mbar_init(&bars->item_empty[i], 10);  // a pair: 4 + 1 warps each; else 8 + 2
     }
     bars->dead = 0;
     fence_mbar_init();
@@ -493,71 +501,71 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       for (int e = rank ? issued : max(0, issued - NS); e < issued; ++e)
         mbar_wait_bounded(&bars->full[e % NS], (e / NS) & 1, a.err, 1u << 22);
     }
-  } else if (warp == 4 * NQ + 1) {
-    // -------------------------------------------------------------------- MMA
+  } else if (warp > 4 * NQ) {
+    // -------------------------------------------------------------------- MMA: a thread per row tile
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16(PAIR ? 2 * kRows : kRows, Cfg::SUB);
+      constexpr uint32_t idesc_s = umma_idesc_bf16(PAIR ? 2 * kRows : kRows, SUB);
       constexpr uint32_t idesc_o = umma_idesc_bf16(PAIR ? 2 * kRows : kRows, Dh) | (1u << 16);  // B (V) is MN-major
-      int e0 = 0, items = 0, work = 0;
-      int g[2] = {0, 0};  // score tiles so far, per row tile
-      int finished[2] = {0, 0};
-      for (;; ++items) {
+      const int w = warp - 4 * NQ - 1;
+      const uint32_t t_s = tmem + 256 + 2 * w * SUB, t_o = tmem + w * Dh;
+      const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes), 16, 1024);
+      int e0 = 0, work = 0, g = 0, finished = 0;  // g: score tiles so far
+      for (int items = 0;; ++items) {
         if (!bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)) break;
         const PromptItem x = bars->item[items & 1];
         mbar_arrive(&bars->item_empty[items & 1]);
         if (x.b < 0) break;
         const PromptTiles ts(x, a, NQ);
-        const int nt = ts.nt;
-        if (nt == 0) continue;
-        const int subs = ts.subs;
-        auto scores = [&](int w, int j, bool last) {  // S = Q_w K^T of score tile j
-          const int buf = (g[w] + j) & 1, t = j / NQ, r0 = (j - t * NQ) * Cfg::SUB;
-          const int e = e0 + pos_k(t), st = e % NS;
-          bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
-          tc_fence_after();
-          const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes), 16, 1024);
-          const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, 16, 1024);
-#pragma unroll
-          for (int k = 0; k < Dh / 16; ++k)
-            mma_ss<PAIR>(tmem + 256 + (2 * w + buf) * Cfg::SUB, qd + (((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4),
-                         kd + (((k >> 2) * (PAIR ? kKeys / 2 : kKeys) * 128 + (k & 3) * 32) >> 4), idesc_s, k != 0);
-          if (last && (j % NQ == NQ - 1 || j + 1 == subs)) mma_commit<PAIR>(&bars->empty[st]);
-          if (last && j + 1 == subs) mma_commit<PAIR>(&bars->q_empty);
-          mma_commit<PAIR>(&bars->s_full[w][buf]);
-        };
-        auto values = [&](int w, int j, bool last) {  // O_w += P V of score tile j
-          const int buf = (g[w] + j) & 1, parity = ((g[w] + j) >> 1) & 1, t = j / NQ, r0 = (j - t * NQ) * Cfg::SUB;
-          const int e = e0 + pos_v(t, nt), st = e % NS;
-          bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
-#pragma unroll
-          for (int hf = 0; hf < Cfg::SUB / 64; ++hf) {  // 64 keys, as the softmax hands them over
-            bar_wait(&bars->dead, &bars->p_full[w][buf][hf], parity, a.err);
+        const int nt = ts.nt, subs = ts.subs;
+        if (nt > 0 && w < ts.chains) {
+          // an entry is free when both row tiles have used it: a lone one answers for the other
+          auto used = [&](uint64_t* bar) {
+            mma_commit<PAIR>(bar);
+            if (NQ == 2 && ts.chains == 1) mma_commit<PAIR>(bar);
+          };
+          auto scores = [&](int j) {  // S = Q K^T of score tile j
+            const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, e = e0 + pos_k(t), st = e % NS;
+            if (r0 == 0) bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
             tc_fence_after();
-            const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + (r0 + hf * 64) * 128, kKeys * 128, 1024);
+            const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, 16, 1024);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ts<PAIR>(tmem + w * Dh, tmem + 256 + (2 * w + buf) * Cfg::SUB + hf * 32 + k * 8, vd + k * (2048 >> 4),
-                           idesc_o, j > 0 || (hf | k) != 0);
+            for (int k = 0; k < Dh / 16; ++k)
+              mma_ss<PAIR>(t_s + buf * SUB, qd + (((k >> 2) * kRows * 128 + (k & 3) * 32) >> 4),
+                           kd + (((k >> 2) * (PAIR ? kKeys / 2 : kKeys) * 128 + (k & 3) * 32) >> 4), idesc_s, k != 0);
+            mma_commit<PAIR>(&bars->s_full[w][buf]);
+            if (j % NQ == NQ - 1 || j + 1 == subs) used(&bars->empty[st]);
+            if (j + 1 == subs) used(&bars->q_empty);
+          };
+          auto values = [&](int j) {  // O += P V of score tile j
+            const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, e = e0 + pos_v(t, nt), st = e % NS;
+            if (r0 == 0) bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+#pragma unroll
+            for (int hf = 0; hf < SUB / 64; ++hf) {  // 64 keys, as the softmax hands them over
+              bar_wait(&bars->dead, &bars->p_full[w][buf][hf], ((g + j) >> 1) & 1, a.err);
+              tc_fence_after();
+              const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + (r0 + hf * 64) * 128, kKeys * 128, 1024);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma_ts<PAIR>(t_o, t_s + buf * SUB + hf * 32 + k * 8, vd + k * (2048 >> 4), idesc_o, j > 0 || (hf | k) != 0);
+            }
+            mma_commit<PAIR>(j + 1 < subs ? &bars->pv[w] : &bars->done[w]);
+            if (j % NQ == NQ - 1 || j + 1 == subs) used(&bars->empty[st]);
+          };
+          bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
+          // S0 S1 | O0 S2 | O1 S3 ...: the next scores are always under way while the softmax works
+          for (int j = 0; j < min(2, subs); ++j) scores(j);
+          for (int j = 0; j < subs; ++j) {
+            values(j);
+            if (j + 2 < subs) scores(j + 2);
           }
-          if (last && (j % NQ == NQ - 1 || j + 1 == subs)) mma_commit<PAIR>(&bars->empty[st]);
-          mma_commit<PAIR>(j + 1 < subs ? &bars->pv[w] : &bars->done[w]);
-        };
-        bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
-        ++work;
-        // per row tile S0 S1 | O0 S2 | O1 S3 ...: the next scores are always under way while the softmax works
-        for (int j = 0; j < min(2, subs); ++j)
-          for (int w = 0; w < ts.chains; ++w) scores(w, j, w == ts.chains - 1);
-        for (int j = 0; j < subs; ++j)
-          for (int w = 0; w < ts.chains; ++w) {
-            values(w, j, w == ts.chains - 1);
-            if (j + 2 < subs) scores(w, j + 2, w == ts.chains - 1);
-          }
+          g += subs;
+          ++finished;
+        }
+        if (nt > 0) ++work;
         e0 += 2 * nt;
-        for (int w = 0; w < ts.chains; ++w) { g[w] += subs; ++finished[w]; }
       }
       // every product is over before the tensor memory is given back
-      for (int w = 0; w < NQ; ++w)
-        if (finished[w] > 0) mbar_wait_bounded(&bars->done[w], (finished[w] - 1) & 1, a.err, 1u << 22);
+      if (finished > 0) mbar_wait_bounded(&bars->done[w], (finished - 1) & 1, a.err, 1u << 22);
     }
     __syncwarp();
   } else if (warp < 4 * NQ) {
@@ -567,6 +575,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     const uint32_t t_o = tmem + lane_base + w * Dh;
     int g = 0, pvs = 0, finished = 0;  // score tiles, phases of pv and of done so far
     int e0 = 0, tails = 0;             // ring entries of the items so far, V tiles cleared
+    bool began = false;
     for (int items = 0;; ++items) {
       if (!__all_sync(0xFFFFFFFFu, PAIR ? bar_wait_cluster(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)
                                         : bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)))
@@ -649,6 +658,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const float neg = m == -INFINITY ? 0.0f : -m;  // nothing seen yet: every weight is 0
         const uint64_t scale2 = f2_pack(a.scale2, a.scale2), neg2 = f2_pack(neg, neg);
         uint64_t sum[2] = {0, 0};
+        if (NQ == 2 && ts.chains == 2) {
+          if (w == 1 || began) turn_wait(w, warp & 3);
+          began = true;
+        }
 #pragma unroll
         for (int c = 0; c < SUB / 32; ++c) {
           uint32_t pk[16];
@@ -674,6 +687,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             }
           }
         }
+        if (NQ == 2 && ts.chains == 2) turn_pass(w, warp & 3);
         float x, y;
         f2_unpack(f2_add(sum[0], sum[1]), x, y);
         l = __fadd_rn(l, __fadd_rn(x, y));
