@@ -15,7 +15,8 @@ namespace qmtp {
 // A group of Dh / 8 lanes owns a row.  Of the rotated dims a lane takes four and their four partners (two loads of
 // 8 bytes), so a pair never leaves its lane; of the others, eight in a row.  A warp takes STEPS steps of
 // 32 / (Dh / 8) head rows of one token, loads them all first and shares the token's angles.  Bound: HBM (one read,
-// one write), with the instructions close behind (an early form of 285 a row step took 129 us where this takes 70).
+// one write), with the instructions close behind: an early form with 285 a row step took 129 us for 15437 tokens,
+// where this takes 73 (5.3 TB/s).
 struct AppendArgs {
   const uint16_t* qkv;
   long long ld;
@@ -28,7 +29,7 @@ struct AppendArgs {
   unsigned* err;
 };
 
-template <int Dh, int STEPS>
+template <int Dh, int STEPS, bool LOOP>
 __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -38,20 +39,25 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
   const int da = turns ? 4 * sub : 8 * sub, db = turns ? half + 4 * sub : 8 * sub + 4;  // this lane's dims: 4 from each on
   const unsigned heads = a.nq + 2 * c.nkv, units = (heads + STEPS * RPS - 1) / (STEPS * RPS);  // warps per token
   const unsigned wid = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int t = wid / units, h0 = (wid - t * units) * STEPS * RPS + lane / LPR;
+  // LOOP: a warp takes a whole token, the next step's rows under way; else one step
+  const int t = LOOP ? wid : wid / units;
+  int h0 = (LOOP ? 0 : wid - t * units) * STEPS * RPS + lane / LPR;
   if (t >= a.T) return;
   const uint16_t* row = a.qkv + (long long)t * a.ld;
-  uint2 x[STEPS][2];
+  uint2 x[STEPS][2], ahead[LOOP ? STEPS : 1][2];
+  auto fetch = [&](uint2 (*to)[2], int first) {
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int h = h0 + i * RPS;
-    x[i][0] = x[i][1] = make_uint2(0, 0);
-    if (h < int(heads)) {
-      const uint16_t* src = row + (a.gated ? (h < a.nq ? 2 * h : a.nq + h) : h) * Dh;
-      x[i][0] = *reinterpret_cast<const uint2*>(src + da);
-      x[i][1] = *reinterpret_cast<const uint2*>(src + db);
+    for (int i = 0; i < STEPS; ++i) {
+      const int h = first + i * RPS;
+      to[i][0] = to[i][1] = make_uint2(0, 0);
+      if (h < int(heads)) {
+        const uint16_t* src = row + (a.gated ? (h < a.nq ? 2 * h : a.nq + h) : h) * Dh;
+        to[i][0] = *reinterpret_cast<const uint2*>(src + da);
+        to[i][1] = *reinterpret_cast<const uint2*>(src + db);
+      }
     }
-  }
+  };
+  fetch(x, h0);
   // the row's sequence and position
   int b, p;
   if (a.cu == nullptr) {
@@ -81,63 +87,74 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
   const uint64_t c2[2] = {f2_pack(cs.x, cs.y), f2_pack(cs.z, cs.w)};
   const uint64_t s2[2] = {f2_pack(sn.x, sn.y), f2_pack(sn.z, sn.w)}, n2[2] = {f2_pack(-sn.x, -sn.y), f2_pack(-sn.z, -sn.w)};
   const long long r0 = cache_row(c, b, 0, p, a.err);  // the position's row of key head 0; a head is a page further
+  for (unsigned u = 0; u < (LOOP ? units : 1u); ++u) {
+    if (LOOP && u + 1 < units) fetch(ahead, h0 + STEPS * RPS);
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int h = h0 + i * RPS;
-    const bool live = h < int(heads), isq = h < a.nq, isv = h >= a.nq + c.nkv;
-    uint2 out[2] = {x[i][0], x[i][1]};
-    const uint16_t* weight = isq ? a.qw : a.kw;
-    if (__any_sync(0xFFFFFFFFu, live && !isv)) {  // values are copied as they are
-      uint64_t y[2][2];
-      uint64_t ss2 = 0;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        y[k][0] = f2_pack(bflo(x[i][k].x), bfhi(x[i][k].x));
-        y[k][1] = f2_pack(bflo(x[i][k].y), bfhi(x[i][k].y));
-        ss2 = f2_fma(y[k][0], y[k][0], ss2);
-        ss2 = f2_fma(y[k][1], y[k][1], ss2);
-      }
-      if (weight != nullptr) {
-        float sa, sb;
-        f2_unpack(ss2, sa, sb);
-        float ss = __fadd_rn(sa, sb);
-#pragma unroll
-        for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
-        const float r = rsqrtf(__fmaf_rn(ss, 1.0f / Dh, a.eps));
-        const uint64_t r2 = f2_pack(r, r);
+    for (int i = 0; i < STEPS; ++i) {
+      const int h = h0 + i * RPS;
+      const bool live = h < int(heads), isq = h < a.nq, isv = h >= a.nq + c.nkv;
+      uint2 out[2] = {x[i][0], x[i][1]};
+      const uint16_t* weight = isq ? a.qw : a.kw;
+      if (__any_sync(0xFFFFFFFFu, live && !isv)) {  // values are copied as they are
+        uint64_t y[2][2];
+        uint64_t ss2 = 0;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint2 w = *reinterpret_cast<const uint2*>(weight + (k ? db : da));
-          y[k][0] = f2_mul(f2_mul(y[k][0], r2), f2_pack(bflo(w.x), bfhi(w.x)));
-          y[k][1] = f2_mul(f2_mul(y[k][1], r2), f2_pack(bflo(w.y), bfhi(w.y)));
+          y[k][0] = f2_pack(bflo(x[i][k].x), bfhi(x[i][k].x));
+          y[k][1] = f2_pack(bflo(x[i][k].y), bfhi(x[i][k].y));
+          ss2 = f2_fma(y[k][0], y[k][0], ss2);
+          ss2 = f2_fma(y[k][1], y[k][1], ss2);
+        }
+        if (weight != nullptr) {
+          float sa, sb;
+          f2_unpack(ss2, sa, sb);
+          float ss = __fadd_rn(sa, sb);
+#pragma unroll
+          for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
+          const float r = rsqrtf(__fmaf_rn(ss, 1.0f / Dh, a.eps));
+          const uint64_t r2 = f2_pack(r, r);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint2 w = *reinterpret_cast<const uint2*>(weight + (k ? db : da));
+            y[k][0] = f2_mul(f2_mul(y[k][0], r2), f2_pack(bflo(w.x), bfhi(w.x)));
+            y[k][1] = f2_mul(f2_mul(y[k][1], r2), f2_pack(bflo(w.y), bfhi(w.y)));
+          }
+        }
+        if (turns) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint64_t u = y[0][k], v = y[1][k];
+            y[0][k] = f2_fma(u, c2[k], f2_mul(v, n2[k]));
+            y[1][k] = f2_fma(v, c2[k], f2_mul(u, s2[k]));
+          }
+        }
+        if (!isv) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float e[4];
+            f2_unpack(y[k][0], e[0], e[1]);
+            f2_unpack(y[k][1], e[2], e[3]);
+            out[k] = make_uint2(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]));
+          }
         }
       }
-      if (turns) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint64_t u = y[0][k], v = y[1][k];
-          y[0][k] = f2_fma(u, c2[k], f2_mul(v, n2[k]));
-          y[1][k] = f2_fma(v, c2[k], f2_mul(u, s2[k]));
-        }
-      }
-      if (!isv) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float e[4];
-          f2_unpack(y[k][0], e[0], e[1]);
-          f2_unpack(y[k][1], e[2], e[3]);
-          out[k] = make_uint2(pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]));
-        }
+      uint16_t* dst = nullptr;
+      if (live && isq)
+        dst = a.q_out + ((long long)t * a.nq + h) * Dh;
+      else if (live && r0 >= 0)
+        dst = (isv ? c.v : c.k) + (r0 + ((long long)(isv ? h - a.nq - c.nkv : h - a.nq) << c.page_log)) * Dh;
+      if (dst) {
+        *reinterpret_cast<uint2*>(dst + da) = out[0];
+        *reinterpret_cast<uint2*>(dst + db) = out[1];
       }
     }
-    uint16_t* dst = nullptr;
-    if (live && isq)
-      dst = a.q_out + ((long long)t * a.nq + h) * Dh;
-    else if (live && r0 >= 0)
-      dst = (isv ? c.v : c.k) + (r0 + ((long long)(isv ? h - a.nq - c.nkv : h - a.nq) << c.page_log)) * Dh;
-    if (dst) {
-      *reinterpret_cast<uint2*>(dst + da) = out[0];
-      *reinterpret_cast<uint2*>(dst + db) = out[1];
+    if (LOOP) {
+      h0 += STEPS * RPS;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        x[i][0] = ahead[LOOP ? i : 0][0];
+        x[i][1] = ahead[LOOP ? i : 0][1];
+      }
     }
   }
 }
@@ -923,20 +940,24 @@ static int launch_decode(const PagedView& v, DecodeArgs a, long long units, cuda
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
 }
 
-template <int Dh, int STEPS>
+template <int Dh, int STEPS, bool LOOP>
 static int launch_append_steps(const PagedView& v, const AppendArgs& a, cudaStream_t st) {
   const int per = STEPS * (32 / (Dh / 8));
-  const long long warps = (long long)a.T * ((a.nq + 2 * v.nkv + per - 1) / per);
-  launch_kernel(paged_append_kernel<Dh, STEPS>, dim3(unsigned((warps + 7) / 8)), dim3(256), 0, st, v, a);
+  const long long warps = LOOP ? a.T : (long long)a.T * ((a.nq + 2 * v.nkv + per - 1) / per);
+  launch_kernel(paged_append_kernel<Dh, STEPS, LOOP>, dim3(unsigned((warps + 7) / 8)), dim3(256), 0, st, v, a);
   return cudaGetLastError() == cudaSuccess ? QMTP_OK : QMTP_ERR_CUDA;
 }
 
 // Few rows: one a lane group, so that none waits for another (3 tokens of 16 + 8 heads of 256: 2.2 us, with four steps a
-// warp 3.5).  Many: four, which share a token's position and angles (15437 tokens: 79 us, with three 87).
+// warp 3.5; 200 tokens 3.6 and 4.1).  More: four steps a warp, which share a token's position and angles (2048 tokens:
+// 11.3 us, with one step 17.1, by whole tokens 16.3).  With 64 tokens an SM and more, whole tokens (15437: 73 us, with four
+// steps 78).
 template <int Dh>
 static int launch_append(const PagedView& v, const AppendArgs& a, cudaStream_t st) {
   const long long groups = (long long)a.T * (a.nq + 2 * v.nkv) * Dh / 256;  // warps of one row step
-  return groups < 32ll * sm_count() ? launch_append_steps<Dh, 1>(v, a, st) : launch_append_steps<Dh, 4>(v, a, st);
+  if (groups < 32ll * sm_count()) return launch_append_steps<Dh, 1, false>(v, a, st);
+  if (a.T < 64 * sm_count()) return launch_append_steps<Dh, 4, false>(v, a, st);
+  return launch_append_steps<Dh, 3, true>(v, a, st);
 }
 
 }  // namespace qmtp

@@ -440,3 +440,14 @@ def test_python_refusals(dev):
         with pytest.raises(ValueError):
             paged.PagedCache(kk, vv)
     no_error()
+
+
+@pytest.mark.parametrize("T", [1, 200, 1000, 10000])
+def test_append_many_rows(T, dev):
+    """Each of the row counts at which the kernel deals its work differently: q, k and v against the formulas."""
+    nq, nkv, dh, rot = 6, 2, 128, 64
+    bt = Batch([(T // 3, T // 3 + 5), (T - T // 3, T - T // 3)], nq, nkv, dh, 64, seed=T)
+    q, k, v, (rq, rqt, rk, rkt, rv) = run_append(bt, dev, True, True, rot, True)
+    assert ((q - rq).abs() <= rqt).all()
+    assert ((k - rk).abs() <= rkt).all()
+    assert torch.equal(v, rv)
