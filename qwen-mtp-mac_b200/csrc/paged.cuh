@@ -127,7 +127,7 @@ __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t
 // waits give up soon too.  False: gave up.
 __device__ __forceinline__ bool bar_wait_slow(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
 #pragma unroll 1
-  for (uint32_t it = 0; it < (1u << 22); ++it) {
+  for (uint32_t it = 0; it < (1u << 20); ++it) {  // seconds
     if (mbar_try_wait(bar, parity)) return true;
     if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(dead)) return false;
   }

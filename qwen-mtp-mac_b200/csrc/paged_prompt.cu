@@ -69,6 +69,9 @@ struct PromptBars {
   uint64_t done[2];  // an item's last product
   uint64_t item_full[2], item_empty[2], next_full;
   uint64_t tail;     // PAIR: this CTA's half of a V tile in which the sequence ends
+  // Two row tiles: the warps of both that share a scheduler take turns at the exponentials.  Side by side they fall into
+  // step, share the exponential unit, and then leave it idle together while they wait and search maxima.
+  uint64_t turn[2][4];
   alignas(16) uint4 next[1];
   PromptItem item[2];
   uint32_t tmem;
@@ -193,14 +196,6 @@ __device__ __forceinline__ void transpose4(uint4 (&v)[4], int lane) {
     }
   }
 }
-// Two row tiles: the warps of both that share a scheduler take turns at the exponentials.  Side by side they fall into
-// step, share the exponential unit and then leave it idle together while they wait and search maxima.
-__device__ __forceinline__ void turn_wait(int w, int quarter) {
-  asm volatile("barrier.cta.sync.aligned %0, 64;" ::"r"(1 + 2 * quarter + w) : "memory");
-}
-__device__ __forceinline__ void turn_pass(int w, int quarter) {
-  asm volatile("barrier.cta.arrive.aligned %0, 64;" ::"r"(1 + 2 * quarter + (w ^ 1)) : "memory");
-}
 // ---- a pair of CTAs (cta_group::2): the MMAs of both are issued by the first; each holds its 128 rows of Q, S, P and O,
 // and half of every K tile (64 keys) and V tile (128 dims), which the tensor cores of both read.
 __device__ __forceinline__ uint32_t in_first_cta(const void* p) {
@@ -286,6 +281,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* s_q = base;
   uint8_t* s_ring = base + NQ * Cfg::q_bytes;
+  static_assert(sizeof(PromptBars) <= 512, "PromptCfg::smem");
   PromptBars* bars = reinterpret_cast<PromptBars*>(s_ring + NS * Cfg::entry);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -308,6 +304,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     mbar_init(&bars->q_empty, NQ);
     mbar_init(&bars->next_full, 1);
     mbar_init(&bars->tail, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&bars->turn[i >> 2][i & 3], 1);
     for (int i = 0; i < 2; ++i) {
       for (int k = 0; k < 2; ++k) {
         mbar_init(&bars->s_full[i][k], 1);
@@ -426,7 +423,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           const int e = e0 + pos, st = e % NS;
           if (!warp_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err)) return;
           // PAIR: the copies of both CTAs count on the first one's barrier; those of a V tile in which the sequence ends
-          // on their own CTA's, whose softmax warps clear it and answer with their weights
+          // on their own CTA's, whose softmax warps clear it and answer with their weights.  The barrier is free again
+          // once the item before (number loads - 2) is done: its last product took every warp's weights.
+          if (PAIR && tail && loads > 1 && !warp_wait(&bars->dead, &bars->done[0], loads & 1, a.err)) return;
           if (lane == 0) {
             if (PAIR && tail) mbar_expect_tx(&bars->tail, Cfg::entry);
             if (PAIR && tail && rank == 0) mbar_arrive(&bars->full[st]);
@@ -575,7 +574,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     const uint32_t t_o = tmem + lane_base + w * Dh;
     int g = 0, pvs = 0, finished = 0;  // score tiles, phases of pv and of done so far
     int e0 = 0, tails = 0;             // ring entries of the items so far, V tiles cleared
-    bool began = false;
+    int turns = 0;
     for (int items = 0;; ++items) {
       if (!__all_sync(0xFFFFFFFFu, PAIR ? bar_wait_cluster(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)
                                         : bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)))
@@ -658,9 +657,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const float neg = m == -INFINITY ? 0.0f : -m;  // nothing seen yet: every weight is 0
         const uint64_t scale2 = f2_pack(a.scale2, a.scale2), neg2 = f2_pack(neg, neg);
         uint64_t sum[2] = {0, 0};
-        if (NQ == 2 && ts.chains == 2) {
-          if (w == 1 || began) turn_wait(w, warp & 3);
-          began = true;
+        if (NQ == 2 && ts.chains == 2) {  // the k-th time: row tile 1 behind tile 0's k-th, tile 0 behind tile 1's (k - 1)-th
+          if (w == 1 || turns > 0) warp_wait(&bars->dead, &bars->turn[w][warp & 3], (turns - 1 + w) & 1, a.err);
+          ++turns;
         }
 #pragma unroll
         for (int c = 0; c < SUB / 32; ++c) {
@@ -687,7 +686,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             }
           }
         }
-        if (NQ == 2 && ts.chains == 2) turn_pass(w, warp & 3);
+        if (NQ == 2 && ts.chains == 2 && lane == 0) mbar_arrive(&bars->turn[w ^ 1][warp & 3]);
         float x, y;
         f2_unpack(f2_add(sum[0], sum[1]), x, y);
         l = __fadd_rn(l, __fadd_rn(x, y));

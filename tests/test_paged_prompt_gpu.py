@@ -233,3 +233,38 @@ def test_prompt_in_a_graph(dev):
         b.replay()
         assert torch.equal(oa, prompt(bt)) and torch.equal(ob, prompt(bt, window=40, sinks=2))
     no_error()
+
+
+@pytest.mark.parametrize("nq,nkv,dh", [(4, 1, 256), (6, 2, 128), (2, 2, 64)])
+def test_prompt_many_short_sequences(nq, nkv, dh, dev):
+    """More items than SMs, a few keys each, so that every block works through many of them one behind the other:
+    one token, chunks that fill one row tile or two, a sequence end in every item."""
+    sizes = [(1 + (i * 7) % 90, 1 + (i * 7) % 90 + (i * 5) % 140) for i in range(250)]
+    bt = Batch(sizes, nq, nkv, dh, 16, seed=dh).put(dev)
+    out = prompt(bt)
+    no_error()
+    check(out, attention_ref(bt))
+    for _ in range(5):
+        assert torch.equal(prompt(bt), out)
+    no_error()
+
+
+def test_pool_beyond_32_bit_offsets(dev):
+    """Pages whose elements lie beyond 2^31 from the pool's start: append, decode and prompt attention there."""
+    from qmtp import paged
+
+    small = Batch([(3, 200), (3, 70)], 4, 2, 256, 64, seed=21)
+    pages = 2 ** 31 // (2 * 64 * 256) + 40
+    cache = paged.PagedCache.empty(pages, 2, 256, 64, dev)
+    first = pages - small.pages
+    cache.k[first:], cache.v[first:] = small.k.to(dev), small.v.to(dev)
+    small.put(dev)
+    table = small.d["table"] + first
+    q, lens, cu = small.d["q"], small.d["lens"], small.d["cu"]
+    assert torch.equal(paged.attention(q, cache, table, lens), paged.attention(*small.args()))
+    assert torch.equal(paged.prompt_attention(q, cache, table, lens, cu), paged.prompt_attention(*small.args(), cu))
+    qkv = torch.randn((6, 8 * 256), device=dev).to(BF16)
+    for c, t in ((cache, table), (small.cache, small.d["table"])):
+        paged.append_qkv(qkv, c, t, lens, n_heads=4)
+    no_error()
+    assert torch.equal(cache.k[first:], small.cache.k) and torch.equal(cache.v[first:], small.cache.v)
