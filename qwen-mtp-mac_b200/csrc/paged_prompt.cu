@@ -674,6 +674,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             // bf16 weights: relative error 2^-9 each, of the size of the output's own rounding; l keeps fp32
             pk[i] = pack_bf16(x, y);
           }
+          // the turn ends with the exponentials: behind the stores the other tile would wait for them too (159 for 154 us)
+          if (NQ == 2 && c == SUB / 32 - 1 && ts.chains == 2 && lane == 0) mbar_arrive(&bars->turn[w ^ 1][warp & 3]);
           tmem_st16(t_s + 16 * c, pk);
           if (c & 1) {  // 64 keys are handed over as soon as they are stored
             tmem_st_wait();
@@ -686,7 +688,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             }
           }
         }
-        if (NQ == 2 && ts.chains == 2 && lane == 0) mbar_arrive(&bars->turn[w ^ 1][warp & 3]);
         float x, y;
         f2_unpack(f2_add(sum[0], sum[1]), x, y);
         l = __fadd_rn(l, __fadd_rn(x, y));
