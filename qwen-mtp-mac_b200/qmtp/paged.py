@@ -15,8 +15,6 @@ the sigmoid output gate of the model's attention layers.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -37,8 +35,7 @@ class PagedCache:
             _tensor(name, t, BF16, self._index)
         _lib.require_cuda(k, v)
         self.pages, self.n_kv, self.page, self.head_dim = k.shape
-        self._base = bytes(_lib.PagedCacheArgs(k=k.data_ptr(), v=v.data_ptr(), pages=self.pages, n_kv=self.n_kv,
-                                               page=self.page, Dh=self.head_dim))
+        self._k_ptr, self._v_ptr = k.data_ptr(), v.data_ptr()
 
     @classmethod
     def empty(cls, pages: int, n_kv: int, head_dim: int, page: int = 64, device="cuda") -> "PagedCache":
@@ -54,17 +51,18 @@ class PagedCache:
     def v(self) -> torch.Tensor:
         return self._v
 
-    def _args(self, table: torch.Tensor, lens: torch.Tensor) -> "_lib.PagedCacheArgs":
+    def _args(self, table: torch.Tensor, lens: torch.Tensor) -> bytes:
         _tensor("table", table, torch.int32, self._index)
         _tensor("lens", lens, torch.int32, self._index)
-        if table.dim() != 2 or lens.dim() != 1:
+        if table.dim() != 2:
             _need(False, "table is [sequences, pages of a sequence], lens [sequences]")
         (B, W), (ld, one) = table.shape, table.stride()
-        if lens.shape[0] != B or W == 0 or (one != 1 and W > 1) or not lens.is_contiguous():
+        if lens.shape != (B,) or W == 0 or (one != 1 and W > 1) or not lens.is_contiguous():
             _need(False, "table is [sequences, pages of a sequence] with contiguous rows, lens [sequences], contiguous")
-        a = _lib.PagedCacheArgs.from_buffer_copy(self._base)
-        a.table, a.lens, a.ld_table, a.table_w, a.B = table.data_ptr(), lens.data_ptr(), ld if B > 1 else W, W, B
-        return a
+        if W > _INT_MAX or B > _INT_MAX:
+            _need(False, "table is too large")
+        return _lib.PAGED_CACHE_ARGS.pack(self._k_ptr, self._v_ptr, table.data_ptr(), lens.data_ptr(), self.pages,
+                                          ld if B > 1 else W, self.n_kv, self.page, self.head_dim, W, B)
 
 
 def _need(ok: bool, what: str) -> None:
@@ -107,13 +105,16 @@ def append_qkv(qkv, cache: PagedCache, table, lens, cu=None, *, n_heads: int, ga
     sequence, and rows at a negative position (lens[b] below the row count), are left as they were."""
     dev, dh = cache._index, cache.head_dim
     _tensor("qkv", qkv, BF16, dev)
-    if qkv.dim() != 2 or qkv.stride(1) != 1:
+    if qkv.dim() != 2:
         _need(False, "qkv is [rows, width] with contiguous rows")
-    T, nq_width = qkv.shape[0], n_heads * (2 if gated else 1) * dh
-    width = nq_width + 2 * cache.n_kv * dh
-    if n_heads < 1 or qkv.shape[1] < width:
+    (T, w), (ld, one) = qkv.shape, qkv.stride()
+    if one != 1:
+        _need(False, "qkv is [rows, width] with contiguous rows")
+    width = (n_heads * (2 if gated else 1) + 2 * cache.n_kv) * dh
+    if n_heads < 1 or w < width:
         _need(False, f"a row of qkv needs {width} values")
-    _check_cu(cu, table.shape[0], dev)
+    if cu is not None:
+        _check_cu(cu, table.shape[0], dev)
     for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
         if w is not None:
             _tensor(name, w, BF16, dev)
@@ -124,69 +125,79 @@ def append_qkv(qkv, cache: PagedCache, table, lens, cu=None, *, n_heads: int, ga
         _need(cos is not None and sin is not None, "cos and sin go together")
         _tensor("cos", cos, torch.float32, dev)
         _tensor("sin", sin, torch.float32, dev)
-        if cos.dim() != 2 or sin.shape != cos.shape or not (cos.is_contiguous() and sin.is_contiguous()):
+        shape = cos.shape
+        if len(shape) != 2 or sin.shape != shape or not (cos.is_contiguous() and sin.is_contiguous()):
             _need(False, "cos and sin are [positions, rotary / 2], contiguous")
-        max_pos, rotary = cos.shape[0], 2 * cos.shape[1]
+        max_pos, rotary = shape[0], 2 * shape[1]
     if out is None:
-        out = qkv.new_empty((T, n_heads, dh))
+        out = qkv.new_empty(T, n_heads, dh)
     else:
         _tensor("out", out, BF16, dev)
         _need(out.shape == (T, n_heads, dh) and out.is_contiguous(), "out is [rows, n_heads, head_dim], contiguous")
     gate = None
     if gated:
-        ld = qkv.stride(0)
         gate = qkv.as_strided((T, n_heads, dh), (ld, 2 * dh, 1), qkv.storage_offset() + dh)
     if T:
         ptr = _lib.ptr
-        _call(dev, "append_qkv", _lib.lib().qmtp_paged_append, qkv.data_ptr(), _row_stride(qkv, width), T, ptr(cu), n_heads,
+        _call(dev, "append_qkv", _lib.lib().qmtp_paged_append, qkv.data_ptr(), _row_stride(T, ld, width), T, ptr(cu), n_heads,
               1 if gated else 0, ptr(q_norm), ptr(k_norm), eps, ptr(cos), ptr(sin), rotary, max_pos, out.data_ptr(),
-              ctypes.byref(cache._args(table, lens)))
+              cache._args(table, lens))
     return out, gate
 
 
-def _row_stride(t, width: int) -> int:
+def _row_stride(rows: int, ld: int, width: int) -> int:
     """Elements between rows; a single row's stride says nothing, so it counts as dense."""
-    return t.stride(0) if t.shape[0] > 1 else -(-width // 8) * 8
+    return ld if rows > 1 else -(-width // 8) * 8
 
 
 def _check_cu(cu, B: int, dev: int) -> None:
-    if cu is not None:
-        _tensor("cu", cu, torch.int32, dev)
-        if cu.shape != (B + 1,) or not cu.is_contiguous():
-            _need(False, "cu is [sequences + 1], contiguous")
+    _tensor("cu", cu, torch.int32, dev)
+    if cu.shape != (B + 1,) or not cu.is_contiguous():
+        _need(False, "cu is [sequences + 1], contiguous")
 
 
 def _attention_args(q, cache: PagedCache, gate, scale, window, sinks, out):
     dev, dh = cache._index, cache.head_dim
     _tensor("q", q, BF16, dev)
-    if q.dim() != 3 or q.shape[2] != dh:
+    if q.dim() != 3:
         _need(False, "q is [rows, heads, head_dim]")
-    (T, nq, _), (ld, hs, one) = q.shape, q.stride()
-    if nq < 1 or one != 1 or (hs != dh and nq > 1) or (ld < nq * dh and T > 1):
+    shape, (ld, hs, one) = q.shape, q.stride()
+    T, nq, d = shape
+    if d != dh:
+        _need(False, "q is [rows, heads, head_dim]")
+    width = nq * dh
+    if nq < 1 or one != 1 or (hs != dh and nq > 1) or (ld < width and T > 1):
         _need(False, "a row of q needs to be contiguous, and rows apart")
     if window < 0 or sinks < 0:
         _need(False, "window and sinks count tokens")
+    if scale is None:
+        scale = dh ** -0.5
+    elif not 0 < scale < 3e38:
+        _need(False, "scale is positive and finite")
+    if T > _INT_MAX or nq > _INT_MAX:
+        _need(False, "q is too large")
     if out is None:
-        out = q.new_empty((T, nq * dh))
+        out = q.new_empty(T, width)
     else:
         _tensor("out", out, BF16, dev)
-        _need(out.shape == (T, nq * dh) and out.is_contiguous(), "out is [rows, heads * head_dim], contiguous")
-    a = _lib.PagedArgs(q.data_ptr(), None, out.data_ptr(), _row_stride(q, nq * dh), 0, 0, T, nq,
-                       dh ** -0.5 if scale is None else scale, min(window, _INT_MAX), min(sinks, _INT_MAX))
+        _need(out.shape == (T, width) and out.is_contiguous(), "out is [rows, heads * head_dim], contiguous")
+    gate_ptr = gate_ld = gate_hs = 0
     if gate is not None:
         _tensor("gate", gate, BF16, dev)
-        ld, hs, one = gate.stride() if gate.dim() == 3 else (0, 0, 0)
-        if gate.shape != q.shape or one != 1:
+        if gate.shape != shape:
             _need(False, "gate has q's shape and contiguous heads")
-        a.gate, a.gate_ld, a.gate_hs = gate.data_ptr(), ld if T > 1 else 0, hs if nq > 1 else 0
-    return a, out
+        gate_ld, gate_hs, gate_one = gate.stride()
+        if gate_one != 1:
+            _need(False, "gate has q's shape and contiguous heads")
+        gate_ptr, gate_ld, gate_hs = gate.data_ptr(), gate_ld if T > 1 else 0, gate_hs if nq > 1 else 0
+    return _lib.PAGED_ARGS.pack(q.data_ptr(), gate_ptr, out.data_ptr(), _row_stride(T, ld, width), gate_ld, gate_hs, T, nq,
+                                scale, min(window, _INT_MAX), min(sinks, _INT_MAX)), out
 
 
 def _launch(cache, what, fn, workspace, a, c, q, *args):
-    pa, pc = ctypes.byref(a), ctypes.byref(c)
-    n = workspace(pa, pc)
+    n = workspace(a, c)
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
-    _call(cache._index, what, fn, pa, *args, pc, _lib.ptr(ws), n)
+    _call(cache._index, what, fn, a, *args, c, _lib.ptr(ws), n)
 
 
 def attention(q, cache: PagedCache, table, lens, *, gate=None, scale: float | None = None, window: int = 0,
@@ -212,6 +223,8 @@ def prompt_attention(q, cache: PagedCache, table, lens, cu, *, gate=None, scale:
     last tokens of sequence b -> bf16 [T, heads * head_dim].  Masks, scale and gate as in ``attention``; rows of
     no sequence are left as they were.  Any number of new tokens per sequence; ``attention`` is the one for a few."""
     a, out = _attention_args(q, cache, gate, scale, window, sinks, out)
+    if cu is None:
+        _need(False, "a prompt's rows are named by cu")
     _check_cu(cu, table.shape[0], cache._index)
     if q.shape[0]:
         L = _lib.lib()

@@ -105,3 +105,13 @@ def test_python_refuses_cpu_tensors():
         paged.PagedCache(x, x.clone())
     with pytest.raises(ValueError):
         paged.PagedCache(x, x[:2])
+
+
+@pytest.mark.parametrize("struct, pack", [("PagedCacheArgs", "PAGED_CACHE_ARGS"), ("PagedArgs", "PAGED_ARGS")])
+def test_packed_arguments_have_the_structures_layout(struct, pack):
+    from qmtp import _lib
+
+    cls = getattr(_lib, struct)
+    values = [float(i) + 0.5 if t is ctypes.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+    got = cls.from_buffer_copy(getattr(_lib, pack).pack(*values))
+    assert [getattr(got, name) for name, _ in cls._fields_] == values

@@ -393,6 +393,22 @@ def test_broadcast_gate_and_huge_window(dev):
     no_error()
 
 
+def test_python_refuses_scales_beyond_fp32_and_missing_rows(dev):
+    from qmtp import paged
+
+    bt = Batch([(2, 70), (2, 40)], 4, 2, 64, 16, seed=13).put(dev)
+    q, cache, table, lens = bt.args()
+    for scale in (1e39, float("inf"), -0.1, 1e-60):
+        with pytest.raises(ValueError):
+            paged.attention(q, cache, table, lens, scale=scale)
+        with pytest.raises(ValueError):
+            paged.prompt_attention(q, cache, table, lens, bt.d["cu"], scale=scale)
+    with pytest.raises(ValueError):
+        paged.prompt_attention(q, cache, table, lens, None)
+    with pytest.raises(ValueError):
+        paged.attention(q, cache, table, lens[:, None])
+
+
 def test_python_refusals(dev):
     from qmtp import paged
 
