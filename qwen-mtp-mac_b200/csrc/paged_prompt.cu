@@ -18,7 +18,7 @@
 // 16384 tokens, 16 / 4 heads of 256, causal: 1361 us, 1.62 PFLOP/s, 2166 cycles a key tile; by single CTAs 1600 us.
 // Dh 128, 64: one CTA, both row tiles, 64 keys a score tile.  Here the exponentials (16 a cycle and SM) take as long as
 // the products, and two warps a scheduler do not hide all of each other's latencies: 6000 tokens, 32 / 8 heads of 128:
-// 287 us, 1.03 PFLOP/s.
+// 283 us, 1.04 PFLOP/s (by turns that pass behind the stores 302).
 #include <algorithm>
 
 #include "paged.cuh"
