@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
           ss2 = f2_fma(y[k][0], y[k][0], ss2);
           ss2 = f2_fma(y[k][1], y[k][1], ss2);
         }
-        if (weight != nullptr) {
+        if (a.qw != nullptr || a.kw != nullptr) {  // the sum by every lane: a step may hold rows with and without a norm
           float sa, sb;
           f2_unpack(ss2, sa, sb);
           float ss = __fadd_rn(sa, sb);
@@ -113,11 +113,13 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
           for (int d = LPR / 2; d >= 1; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
           const float r = rsqrtf(__fmaf_rn(ss, 1.0f / Dh, a.eps));
           const uint64_t r2 = f2_pack(r, r);
+          if (weight != nullptr) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint2 w = *reinterpret_cast<const uint2*>(weight + (k ? db : da));
-            y[k][0] = f2_mul(f2_mul(y[k][0], r2), f2_pack(bflo(w.x), bfhi(w.x)));
-            y[k][1] = f2_mul(f2_mul(y[k][1], r2), f2_pack(bflo(w.y), bfhi(w.y)));
+            for (int k = 0; k < 2; ++k) {
+              const uint2 w = *reinterpret_cast<const uint2*>(weight + (k ? db : da));
+              y[k][0] = f2_mul(f2_mul(y[k][0], r2), f2_pack(bflo(w.x), bfhi(w.x)));
+              y[k][1] = f2_mul(f2_mul(y[k][1], r2), f2_pack(bflo(w.y), bfhi(w.y)));
+            }
           }
         }
         if (turns) {

@@ -1,0 +1,46 @@
+"""Edges of the paged-cache operators (qmtp.paged): optional arguments on their own, infinities and NaN in every
+place, row offsets that are no offsets.  64-bit references and tolerances as in _paged_ref."""
+import pytest
+import torch
+
+from tests._paged_ref import BF16, Batch, append_ref, attention_ref, check
+
+pytestmark = pytest.mark.gpu
+
+
+def device_error():
+    from qmtp import _lib
+
+    torch.cuda.synchronize()
+    return _lib.device_error()
+
+
+# ------------------------------------------------------------------------------------ append
+@pytest.mark.parametrize("nq,nkv,dh,rotary,gated", [
+    (7, 1, 128, 48, True), (5, 5, 64, 64, True), (3, 1, 64, 0, False), (16, 4, 256, 64, True), (6, 2, 64, 32, False)])
+@pytest.mark.parametrize("norm", ["q", "k"])
+@pytest.mark.parametrize("T", [5, 400, 9600])
+def test_append_with_one_norm(nq, nkv, dh, rotary, gated, norm, T, dev):
+    """A norm of the queries alone, and of the keys alone: a warp's step holds rows with a norm beside rows without one
+    where the query heads do not fill it; by each of the ways that the kernel deals rows."""
+    from qmtp import paged
+
+    n = T // 5
+    bt = Batch([(n, n + 3), (T - n, T - n + 17)], nq, nkv, dh, 32, seed=T + dh)
+    width = (nq * (2 if gated else 1) + 2 * nkv) * dh
+    qkv = torch.randn((T, width), generator=bt.g).to(BF16)
+    w = (1 + 0.3 * torch.randn(dh, generator=bt.g)).to(BF16)
+    qn, kn = (w, None) if norm == "q" else (None, w)
+    cos = sin = None
+    if rotary:
+        ang = torch.arange(T + 20)[:, None] * 1e4 ** (-torch.arange(rotary // 2) / (rotary // 2))
+        cos, sin = ang.cos().float(), ang.sin().float()
+    rq, rqt, rk, rkt, rv = append_ref(bt, qkv, gated, qn, kn, cos, sin, 1e-6)
+    bt.put(dev)
+    dd = lambda t: None if t is None else t.to(dev)
+    q, _ = paged.append_qkv(qkv.to(dev), bt.cache, bt.d["table"], bt.d["lens"], bt.d["cu"], n_heads=nq, gated=gated,
+                            q_norm=dd(qn), k_norm=dd(kn), cos=dd(cos), sin=dd(sin))
+    assert device_error() == 0
+    assert ((q.cpu().double() - rq).abs() <= rqt).all()
+    assert ((bt.cache.k.cpu().double() - rk).abs() <= rkt).all()
+    assert torch.equal(bt.cache.v.cpu().double(), rv)
