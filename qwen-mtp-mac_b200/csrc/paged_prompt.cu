@@ -792,7 +792,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (a.splits > 1) {
             a.ws_o[(long long)x.split * a.T * a.nq * Dh + at] = oo[e];
           } else {
-            float y = __fdiv_rn(oo[e], ll);
+            float y = ll == 0.0f ? 0.0f : __fdiv_rn(oo[e], ll);  // nothing seen: zeros
             if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[tr * a.gate_ld + hh * a.gate_hs + d])));
             a.out[at] = f2bf(y);
           }

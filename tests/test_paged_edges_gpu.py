@@ -44,3 +44,34 @@ def test_append_with_one_norm(nq, nkv, dh, rotary, gated, norm, T, dev):
     assert ((q.cpu().double() - rq).abs() <= rqt).all()
     assert ((bt.cache.k.cpu().double() - rk).abs() <= rkt).all()
     assert torch.equal(bt.cache.v.cpu().double(), rv)
+
+
+# ------------------------------------------------------------------------------------ attention
+def set_value(bt, b, pos, dim, value):
+    """V of position pos of sequence b, every key head: value at dim."""
+    pg, sl = bt.rows(b, pos)
+    bt.v[pg, :, sl, dim] = value
+
+
+@pytest.mark.parametrize("table_extra", [0, 200])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dh", [256, 128, 64])
+def test_prompt_rows_before_the_sequence_are_zeros(dh, poison, table_extra, dev):
+    """A chunk longer than its sequence: its first rows see no key and give zeros, whatever the values in their tile are;
+    with a wide table the keys are split and joined."""
+    from qmtp import paged
+
+    bt = Batch([(5, 2), (40, 33)], 4, 2, dh, 16, seed=dh, table_extra=table_extra)
+    ref = attention_ref(bt)
+    for b in range(2):
+        set_value(bt, b, 0, 5, poison)
+    bt.put(dev)
+    out = paged.prompt_attention(*bt.args(), bt.d["cu"], gate=bt.d["gate"][:, :, 1]).cpu()
+    assert device_error() == 0
+    unseen = torch.tensor([True] * 3 + [False] * 2 + [True] * 7 + [False] * 33)
+    assert (out[unseen] == 0).all()
+    heads = out.view(-1, 4, dh)
+    assert not torch.isfinite(heads[~unseen][..., 5]).any()
+    rest = torch.arange(dh) != 5
+    cut = lambda t: t.view(-1, 4, dh)[..., rest].reshape(t.shape[0], -1)
+    check(cut(out), (cut(ref[0]), cut(ref[1])))
