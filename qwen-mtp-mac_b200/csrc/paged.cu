@@ -664,6 +664,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       // class k: slab number k of the first ones (few calls have any), and the one of the others with that residue
       float m1[16], l1[16];
       int part_of[16];
+      unsigned absent = 0;
       float M = kNone;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -671,7 +672,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         part_of[k] = pt < n_parts ? pt : 0;
         m1[k] = ld_dsmem(mlp, part_of[k]);
         l1[k] = ld_dsmem(mlp + 1, part_of[k]);
-        if (pt >= n_parts) m1[k] = kNone;
+        if (pt >= n_parts) {  // a class without a slab adds nothing, whatever the slab read in its place holds
+          m1[k] = kNone;
+          l1[k] = 0.0f;
+          absent |= 1u << k;
+        }
         M = fmaxf(M, m1[k]);
       }
       for (int k = 0; k < mine_slabs.first; ++k) M = fmaxf(M, ld_dsmem(mlp, k));
@@ -680,7 +685,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       for (int k0 = 0; k0 < 16; k0 += 8) {
         float4 v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = ld_dsmem_v4(op, part_of[k0 + k]);
+        for (int k = 0; k < 8; ++k) {
+          v[k] = ld_dsmem_v4(op, part_of[k0 + k]);
+          if (absent >> (k0 + k) & 1) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);  // 0 times an infinity would be NaN
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float z[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.0f;
@@ -713,7 +721,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
 // is its number mod 16; every class is summed in rising order, then the classes in order, so the order of
 // additions belongs to the slabs' positions, however they are dealt to threads.  Two ways to deal them:
 //   wide (few rows): a block per (row, 64 dims), 16 threads of 4 dims for each class;
-//   warp (many rows): a warp per (row, 128 dims), 4 dims a lane and every class in its registers, no barrier.
+//   warp (many rows): a warp per (row, 128 dims), 4 dims a lane and every class in its registers, no barrier; four blocks
+//   an SM (24 x 3 tokens, window 1024: 32.3 us, with 137 registers and three blocks 34.5).
 struct JoinRow {
   const float2* ml;   // slab i at ml[i * stride]
   const float* o;     // ... at o[i * stride * Dh]
@@ -788,7 +797,7 @@ __global__ void __launch_bounds__(256) paged_join_wide_kernel(PagedView c, Decod
 }
 
 template <int Dh>
-__global__ void __launch_bounds__(128) paged_join_warp_kernel(PagedView c, DecodeArgs a) {
+__global__ void __launch_bounds__(128, 4) paged_join_warp_kernel(PagedView c, DecodeArgs a) {
   pdl_wait();
   constexpr int LPR = Dh / 4, RPW = LPR < 32 ? 32 / LPR : 1, WPR = LPR > 32 ? LPR / 32 : 1;  // lanes a row, rows a warp
   const int lane = threadIdx.x & 31, wid = blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -824,15 +833,17 @@ __global__ void __launch_bounds__(128) paged_join_warp_kernel(PagedView c, Decod
       for (int h = 0; h < 16; h += 8) {
         float4 x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // eight loads under way at once; a number outside the list has weight 0
+        for (int k = 0; k < 8; ++k)  // eight loads under way at once; numbers outside the list read a listed slab
           x[k] = *reinterpret_cast<const float4*>(po + min(max(i + h + k, 0), j.sl.count - 1) * step);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float wk = __shfl_sync(0xFFFFFFFFu, w, half + h + k);
-          acc[h + k].x = __fmaf_rn(wk, x[k].x, acc[h + k].x);
-          acc[h + k].y = __fmaf_rn(wk, x[k].y, acc[h + k].y);
-          acc[h + k].z = __fmaf_rn(wk, x[k].z, acc[h + k].z);
-          acc[h + k].w = __fmaf_rn(wk, x[k].w, acc[h + k].w);
+          if (i + h + k >= i0 && i + h + k < i1) {  // ... and add nothing: 0 times an infinity would be NaN
+            acc[h + k].x = __fmaf_rn(wk, x[k].x, acc[h + k].x);
+            acc[h + k].y = __fmaf_rn(wk, x[k].y, acc[h + k].y);
+            acc[h + k].z = __fmaf_rn(wk, x[k].z, acc[h + k].z);
+            acc[h + k].w = __fmaf_rn(wk, x[k].w, acc[h + k].w);
+          }
         }
       }
     }

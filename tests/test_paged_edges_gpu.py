@@ -75,3 +75,34 @@ def test_prompt_rows_before_the_sequence_are_zeros(dh, poison, table_extra, dev)
     rest = torch.arange(dh) != 5
     cut = lambda t: t.view(-1, 4, dh)[..., rest].reshape(t.shape[0], -1)
     check(cut(out), (cut(ref[0]), cut(ref[1])))
+
+
+@pytest.mark.parametrize("dh,nq,nkv,S", [(64, 4, 2, 2), (128, 4, 2, 1), (256, 4, 2, 3)])
+@pytest.mark.parametrize("length,window,sinks", [(100, 0, 0), (1000, 0, 0), (2048, 0, 0), (1500, 600, 300), (3500, 0, 0)])
+def test_decode_infinite_value_in_any_slab(dh, nq, nkv, S, length, window, sinks, dev):
+    """An infinite value that is seen gives an infinity in its dim and leaves the others, in whichever slab of keys it lies
+    and by each form of the join, which agree bit for bit: in one launch (short tables), a block a row (few rows), a
+    warp a row (many)."""
+    from qmtp import paged
+
+    bt = Batch([(S, length)], nq, nkv, dh, 64, seed=length + dh).put(dev)
+    q, cache, table, lens = bt.args()
+    wide = torch.full((1, 1000), -1, dtype=torch.int32, device=dev)
+    wide[:, : table.shape[1]] = table
+    many = 1 + 2 * 148 // (S * nq)
+    kw = dict(window=window, sinks=sinks)
+    seen = [j for j in range(0, length - S + 1, 128) if not window or j < sinks or length - S - j < window] + [length - S]
+    for j in seen:
+        pg, sl = bt.rows(0, j)
+        for value in (float("inf"), float("-inf")):
+            held = cache.v[pg, :, sl, 5].clone()
+            cache.v[pg, :, sl, 5] = value
+            short = paged.attention(q, cache, table, lens, **kw)
+            block = paged.attention(q, cache, wide, lens, **kw)
+            warp = paged.attention(q.repeat(many, 1, 1), cache, wide.repeat(many, 1), lens.repeat(many), **kw)
+            cache.v[pg, :, sl, 5] = held
+            heads = short.view(S, nq, dh)
+            assert (heads[..., 5] == value).all(), (j, value)
+            assert torch.isfinite(heads[..., :5]).all() and torch.isfinite(heads[..., 6:]).all(), (j, value)
+            assert torch.equal(short, block) and torch.equal(warp, block.repeat(many, 1)), (j, value)
+    assert device_error() == 0
