@@ -22,6 +22,7 @@
 #include <algorithm>
 
 #include "paged.cuh"
+#include "prompt_items.cuh"
 
 namespace qmtp {
 
@@ -334,10 +335,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     const int TT = 2 * a.tpt;                                             // tokens per item
     const int box = min(1 << c.page_log, Cfg::box), parts = kKeys / box;  // rows per box, boxes down a tile
     const long long none = (c.pages * c.nkv) << c.page_log;                // past the end: reads as zeros
-    int seq = 0, before = 0;  // sequences [0, seq) hold `before` row tiles: items come in rising order
-    int e0 = 0, issued = 0, loads = 0, tails = 0;
+    ItemCursor at_seq;
+    int e0 = 0, issued = 0, loads = 0, tails = 0, asked = 0;
     long long u = blockIdx.x / (PAIR ? 2 : 1);
-    for (int i = 0;; ++i) {
+    bool own = true;  // the block's own place, not one that it took over
+    for (int i = 0;;) {
       // The next item: that of a block of the grid that has not started, taken over while this one runs.  With no more
       // blocks than SMs each finds a place of its own, and none is taken.
       if (lane == 0 && rank == 0 && a.takes_over) {
@@ -349,8 +351,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       x.split = int(u % a.splits);
       x.kh = int(u / a.splits % c.nkv);
       const long long tile = u / a.splits / c.nkv;
-      while ((rank == 0 || i == 0) && seq < c.B) {
-        const int k = seq + lane;
+      at_seq.seek(tile);
+      while ((rank == 0 || own) && at_seq.seq < c.B) {
+        const int k = at_seq.seq + lane;
         int n = 0, c0 = 0, len = 0;
         if (k < c.B) {
           c0 = a.cu[k];
@@ -369,26 +372,31 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           const int y = __shfl_up_sync(0xFFFFFFFFu, incl, d);
           if (lane >= d) incl += y;
         }
-        const long long at = tile - before - (incl - tiles);
+        const long long at = tile - at_seq.before - (incl - tiles);
         const unsigned hit = __ballot_sync(0xFFFFFFFFu, at >= 0 && at < tiles);
         if (hit) {
           const int src = __ffs(hit) - 1;
-          x.b = seq + src;
+          x.b = at_seq.seq + src;
           x.n = __shfl_sync(0xFFFFFFFFu, n, src);
           x.c0 = __shfl_sync(0xFFFFFFFFu, c0, src);
           x.len = __shfl_sync(0xFFFFFFFFu, len, src);
           x.tok0 = (__shfl_sync(0xFFFFFFFFu, tiles, src) - 1 - int(__shfl_sync(0xFFFFFFFFu, int(at), src))) * TT;
           break;
         }
-        before += __shfl_sync(0xFFFFFFFFu, incl, 31);
-        seq += 32;
+        at_seq.pass(32, __shfl_sync(0xFFFFFFFFu, incl, 31));
       }
+      auto take_over = [&] {  // the block that the request of this round has got, or -1
+        int next = -1;
+        if (a.takes_over && bar_wait(&bars->dead, &bars->next_full, asked & 1, a.err)) next = next_block(bars->next);
+        ++asked;
+        return __shfl_sync(0xFFFFFFFFu, next, 0);
+      };
       auto hand_out = [&](const PromptItem& y, int at) {
         const bool ok = warp_wait(&bars->dead, &bars->item_empty[at & 1], ((at >> 1) & 1) ^ 1, a.err);
         if (lane == 0) {
           bars->item[at & 1] = y;
           mbar_arrive(&bars->item_full[at & 1]);
-          if (PAIR && rank == 0 && at > 0) {
+          if (PAIR && rank == 0 && (!own || y.b < 0)) {
             const uint32_t to = in_cta(&bars->item[at & 1], 1);
             const int v[7] = {y.b, y.kh, y.split, y.tok0, y.n, y.c0, y.len};
 #pragma unroll
@@ -399,10 +407,20 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         __syncwarp();
         return ok;
       };
+      if (rank == 0 && x.b < 0) {  // a place without rows (the grid has as many as there can be): on with the next
+        const int next = take_over();
+        if (next >= 0) {
+          u = next / (PAIR ? 2 : 1);
+          own = false;
+          continue;
+        }
+        hand_out(x, i);
+        break;
+      }
       bool ok;
-      if (rank == 0 || i == 0) {
+      if (rank == 0 || (own && x.b >= 0)) {
         ok = hand_out(x, i);
-      } else {  // the second CTA finds the first item itself and is told of the others
+      } else {  // the second CTA finds the block's own item itself and is told of the others
         ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(&bars->dead, &bars->item_full[i & 1], (i >> 1) & 1, a.err));
         if (!ok) break;
         x = bars->item[i & 1];
@@ -479,22 +497,23 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         }
         e0 += 2 * ts.nt;
       }
+      ++i;
+      own = false;
       if (rank == 1) {
         if (x.b < 0) break;
         continue;
       }
-      int next = -1;
-      if (a.takes_over && bar_wait(&bars->dead, &bars->next_full, i & 1, a.err)) next = next_block(bars->next);
-      next = __shfl_sync(0xFFFFFFFFu, next, 0);
-      if (x.b < 0 || !ok) break;
+      const int next = take_over();
+      if (!ok) break;
       if (next < 0) {
         x.b = -1;
-        hand_out(x, i + 1);
+        hand_out(x, i);
         break;
       }
       u = next / (PAIR ? 2 : 1);
     }
     if (*reinterpret_cast<volatile int*>(&bars->dead)) {  // copies in flight end before the CTA does
+      if (a.takes_over && asked > 0) mbar_wait_bounded(&bars->next_full, (asked - 1) & 1, a.err, 1u << 22);
       if (tails > 0) mbar_wait_bounded(&bars->tail, (tails - 1) & 1, a.err, 1u << 22);
       if (loads > 0 && rank == 0) mbar_wait_bounded(&bars->q_full, (loads - 1) & 1, a.err, 1u << 22);
       for (int e = rank ? issued : max(0, issued - NS); e < issued; ++e)

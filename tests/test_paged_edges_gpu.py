@@ -106,3 +106,23 @@ def test_decode_infinite_value_in_any_slab(dh, nq, nkv, S, length, window, sinks
             assert torch.isfinite(heads[..., :5]).all() and torch.isfinite(heads[..., 6:]).all(), (j, value)
             assert torch.equal(short, block) and torch.equal(warp, block.repeat(many, 1)), (j, value)
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("nq,nkv,dh", [(16, 4, 256), (8, 4, 128), (4, 4, 64)])
+def test_prompt_call_with_far_more_places_than_rows(nq, nkv, dh, dev):
+    """Most of q's rows belong to no sequence and most sequences have no new token: the blocks' places without rows lie
+    between, before and behind those with rows."""
+    from qmtp import paged
+
+    sizes = [(0, 3)] * 70 + [(90, 90)] + [(0, 0)] * 60 + [(1, 200), (130, 400)] + [(0, 1)] * 100 + [(33, 30), (0, 9)]
+    bt = Batch(sizes, nq, nkv, dh, 16, seed=dh).put(dev)
+    ref = attention_ref(bt, gate=False)
+    T, first = 20000, 12345
+    q = torch.full((T, nq, dh), float("nan"), dtype=BF16, device=dev)
+    q[first: first + bt.T] = bt.d["q"]
+    for _ in range(3):
+        out = torch.full((T, nq * dh), 3.0, dtype=BF16, device=dev)
+        paged.prompt_attention(q, bt.cache, bt.d["table"], bt.d["lens"], bt.d["cu"] + first, out=out)
+        assert device_error() == 0
+        assert (out[:first] == 3).all() and (out[first + bt.T:] == 3).all()
+        check(out[first: first + bt.T], ref)
