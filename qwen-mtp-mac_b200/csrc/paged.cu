@@ -265,12 +265,13 @@ struct DecodeSmem {
 };
 
 __device__ __forceinline__ float join_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M)); }
-// Four dims of a finished row: sum / denominator, the gate, one rounding.
-__device__ __forceinline__ void join_store(const DecodeArgs& a, float (&y)[4], float ll, uint2 gate, uint16_t* dst) {
+// Four dims of a finished row: sum / denominator (0 where the row sees no key; 0 / 0 = NaN where every score that it sees
+// is -inf), the gate, one rounding.
+__device__ __forceinline__ void join_store(const DecodeArgs& a, float (&y)[4], float ll, bool sees, uint2 gate, uint16_t* dst) {
   const float g[4] = {bflo(gate.x), bfhi(gate.x), bflo(gate.y), bfhi(gate.y)};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    y[k] = ll == 0.0f ? 0.0f : __fdiv_rn(y[k], ll);
+    y[k] = sees ? __fdiv_rn(y[k], ll) : 0.0f;
     if (a.gate) y[k] = __fmul_rn(y[k], sigmoid_f32(g[k]));
   }
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
@@ -710,7 +711,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
           ll = __fadd_rn(ll, den);
         }
       }
-      join_store(a, y, ll, g2, a.out + (t * a.nq + h) * Dh + d);
+      join_store(a, y, ll, mine.len - a.S + s >= 0, g2, a.out + (t * a.nq + h) * Dh + d);
     }
     __syncwarp();
     cluster_sync_all();  // the others have read this CTA's shared memory
@@ -728,12 +729,15 @@ struct JoinRow {
   const float* o;     // ... at o[i * stride * Dh]
   long long out, gate, stride;
   SlabList sl;
+  bool sees;  // the row's position is one of the sequence, so it sees at least its own key
 };
 template <int Dh>
 __device__ __forceinline__ JoinRow join_row(const PagedView& c, const DecodeArgs& a, int br) {
   JoinRow j;
   const int rows = a.S * a.nq, b = br / rows, r = br - b * rows, s = r / a.nq, h = r - s * a.nq;
-  j.sl = slab_list(a, seq_len(c, b, nullptr));
+  const int len = seq_len(c, b, nullptr);
+  j.sl = slab_list(a, len);
+  j.sees = len - a.S + s >= 0;
   j.ml = a.ws_ml + (long long)b * a.max_slabs * rows + r;
   j.o = a.ws_o + ((long long)b * a.max_slabs * rows + r) * Dh;
   j.stride = rows;
@@ -791,7 +795,7 @@ __global__ void __launch_bounds__(256) paged_join_wide_kernel(PagedView c, Decod
     y = __fadd_rn(y, so[i * 64 + tid]);
     ll = __fadd_rn(ll, s_l[i]);
   }
-  y = ll == 0.0f ? 0.0f : __fdiv_rn(y, ll);
+  y = j.sees ? __fdiv_rn(y, ll) : 0.0f;
   if (a.gate) y = __fmul_rn(y, sigmoid_f32(gate));
   a.out[j.out + d0 + tid] = f2bf(y);
 }
@@ -857,7 +861,7 @@ __global__ void __launch_bounds__(128, 4) paged_join_warp_kernel(PagedView c, De
     y[3] = __fadd_rn(y[3], acc[k].w);
     ll = __fadd_rn(ll, __shfl_sync(0xFFFFFFFFu, den, half + k));
   }
-  if (live) join_store(a, y, ll, g2, a.out + j.out + d);
+  if (live) join_store(a, y, ll, j.sees, g2, a.out + j.out + d);
 }
 
 // ----------------------------------------------------------------------------- host

@@ -739,7 +739,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       }
       // O / l, gate, store; a row with an infinity or NaN is settled by the definition afterwards
       const long long orow = (row * a.nq + h) * Dh;
-      const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+      const float inv = p < 0 ? 0.0f : __fdiv_rn(1.0f, l);  // l = 0 at p >= 0: every score seen is -inf, 0 / 0
       float* part = a.ws_o + (long long)x.split * a.T * a.nq * Dh + orow;
       float probe[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // 0 unless O holds an infinity or NaN
 #pragma unroll 2  // not more: code that runs once an item costs instruction fetches (8 chunks unrolled: +2 us)
@@ -811,7 +811,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (a.splits > 1) {
             a.ws_o[(long long)x.split * a.T * a.nq * Dh + at] = oo[e];
           } else {
-            float y = ll == 0.0f ? 0.0f : __fdiv_rn(oo[e], ll);  // nothing seen: zeros
+            float y = x.len - x.n + ti < 0 ? 0.0f : __fdiv_rn(oo[e], ll);  // nothing seen: zeros
             if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[tr * a.gate_ld + hh * a.gate_hs + d])));
             a.out[at] = f2bf(y);
           }
@@ -842,12 +842,16 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedView c, PromptArg
   const long long rh = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (long long)a.T * a.nq;
   if (rh >= rows) return;
   const int row = int(rh / a.nq), h = int(rh - (long long)row * a.nq);
-  bool mine = false;
+  bool mine = false, sees = false;  // the row is one of a sequence; its position is one, so it sees at least its own key
   for (int i = 0; i < c.B; i += 32) {
     const int k = i + lane;
-    mine |= k < c.B && a.cu[k] >= 0 && a.cu[k + 1] <= a.T && a.cu[k] <= row && row < a.cu[k + 1];
+    if (k < c.B && a.cu[k] >= 0 && a.cu[k + 1] <= a.T && a.cu[k] <= row && row < a.cu[k + 1]) {
+      mine = true;
+      sees = seq_len(c, k, nullptr) - a.cu[k + 1] + row >= 0;
+    }
   }
   if (!__any_sync(0xFFFFFFFFu, mine)) return;
+  sees = __any_sync(0xFFFFFFFFu, sees);
   float M = -INFINITY, l = 0.0f, o[N] = {};
   for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.ws_ml[s * rows + rh].x);
   const float safe = M == -INFINITY ? 0.0f : M;
@@ -862,7 +866,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PagedView c, PromptArg
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const int d = lane + 32 * e;
-    float y = l == 0.0f ? 0.0f : __fdiv_rn(o[e], l);
+    float y = sees ? __fdiv_rn(o[e], l) : 0.0f;
     if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[row * a.gate_ld + h * a.gate_hs + d])));
     a.out[rh * Dh + d] = f2bf(y);
   }

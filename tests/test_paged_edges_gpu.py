@@ -126,3 +126,28 @@ def test_prompt_call_with_far_more_places_than_rows(nq, nkv, dh, dev):
         assert device_error() == 0
         assert (out[:first] == 3).all() and (out[first + bt.T:] == 3).all()
         check(out[first: first + bt.T], ref)
+
+
+@pytest.mark.parametrize("table_extra", [0, 300])
+@pytest.mark.parametrize("dh,nq,nkv,copies", [(64, 4, 2, 1), (128, 4, 2, 1), (256, 4, 2, 1), (64, 4, 2, 60), (256, 4, 2, 60)])
+def test_scores_of_minus_infinity(dh, nq, nkv, copies, table_extra, dev):
+    """A key whose score is -inf has weight 0; a query that sees only such keys has no softmax (0 / 0) and gives NaN, as the
+    definition does, while one that sees no key gives zeros."""
+    from qmtp import paged
+
+    S = 3
+    sizes = [(S, 1), (S, 2), (S, 500), (S, 300)] * copies
+    bt = Batch(sizes, nq, nkv, dh, 16, seed=dh, table_extra=table_extra)
+    bt.q[:, :, 0] = 1.0
+    for b, (_, length) in enumerate(bt.sizes):
+        pg, sl = bt.rows(b, torch.arange(length if b % 4 == 3 else 1))
+        bt.k[pg, :, sl, 0] = float("-inf")
+    ref = attention_ref(bt, gate=False)
+    bt.put(dev)
+    # sequence 0 sees its one key, sequence 1 that key and then a second one, 2 four hundred others, 3 only such keys
+    kind = torch.tensor([0, 0, 1, 0, 1, 2, 2, 2, 2, 1, 1, 1] * copies)  # 0: no key, 1: NaN, 2: the reference
+    for out in (paged.attention(*bt.args()), paged.prompt_attention(*bt.args(), bt.d["cu"])):
+        out = out.cpu()
+        assert (out[kind == 0] == 0).all() and torch.isnan(out[kind == 1]).all()
+        check(out, ref, rows=kind == 2)
+    assert device_error() == 0
