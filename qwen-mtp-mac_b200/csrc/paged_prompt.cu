@@ -536,11 +536,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const PromptTiles ts(x, a, NQ);
         const int nt = ts.nt, subs = ts.subs;
         if (nt > 0 && w < ts.chains) {
-          // an entry is free when both row tiles have used it: a lone one answers for the other
-          auto used = [&](uint64_t* bar) {
-            mma_commit<PAIR>(bar);
-            if (NQ == 2 && ts.chains == 1) mma_commit<PAIR>(bar);
-          };
+          auto used = [&](uint64_t* bar) { mma_commit<PAIR>(bar); };  // an entry is free when both row tiles have used it
           auto scores = [&](int j) {  // S = Q K^T of score tile j
             const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, e = e0 + pos_k(t), st = e % NS;
             if (r0 == 0) bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
@@ -578,6 +574,16 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           }
           g += subs;
           ++finished;
+        } else if (nt > 0) {
+          // A row tile without tokens: its thread follows the item's barriers all the same.  A wait by parity is only right
+          // for the phase after the last one that its thread has seen: behind a skipped item it could pass while the item's own
+          // copies were under way, and the next one's products read tiles that were not there.
+          bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
+          mbar_arrive(&bars->q_empty);
+          for (int e = e0; e < e0 + 2 * nt; ++e) {
+            bar_wait(&bars->dead, &bars->full[e % NS], (e / NS) & 1, a.err);
+            mbar_arrive(&bars->empty[e % NS]);
+          }
         }
         if (nt > 0) ++work;
         e0 += 2 * nt;

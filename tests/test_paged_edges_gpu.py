@@ -151,3 +151,25 @@ def test_scores_of_minus_infinity(dh, nq, nkv, copies, table_extra, dev):
         assert (out[kind == 0] == 0).all() and torch.isnan(out[kind == 1]).all()
         check(out, ref, rows=kind == 2)
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("nq,nkv,dh", [(4, 1, 256), (6, 2, 128), (8, 2, 128), (2, 2, 64)])
+def test_prompt_lone_and_paired_row_tiles_in_turn(nq, nkv, dh, dev):
+    """Chunks of one row tile and of two follow one another in every block, a few key tiles each: the same bits every time,
+    with what the kernel reads in the caches and not, and those of each sequence by itself."""
+    from qmtp import paged
+
+    sizes = [(1 + (i * 7) % 90, 1 + (i * 7) % 90 + (i * 5) % 140) for i in range(250)]
+    bt = Batch(sizes, nq, nkv, dh, 16, seed=dh).put(dev)
+    flush = torch.empty(64 << 20, dtype=torch.int32, device=dev)
+    alone = [paged.prompt_attention(bt.d["q"][c:c + n], bt.cache, bt.d["table"][b:b + 1], bt.d["lens"][b:b + 1],
+                                    torch.tensor([0, n], dtype=torch.int32, device=dev))
+             for b, ((n, _), c) in enumerate(zip(sizes, bt.cu.tolist()))]
+    alone = torch.cat(alone)
+    wrong = torch.zeros(300, dtype=torch.bool, device=dev)
+    for i in range(300):
+        if i % 3 == 0:
+            flush.fill_(i)
+        wrong[i] = (paged.prompt_attention(*bt.args(), bt.d["cu"]) != alone).any()
+    assert device_error() == 0
+    assert not wrong.any(), int(wrong.sum())
