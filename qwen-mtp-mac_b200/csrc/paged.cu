@@ -261,7 +261,7 @@ struct DecodeSmem {
   uint64_t full[Cfg::ring], empty[Cfg::ring], q_full[2], q_empty[2];
   int bad[2];
   int scan[8];
-  int dead;
+  WaitState wait;
 };
 
 __device__ __forceinline__ float join_weight(float m, float M) { return m == -INFINITY ? 0.0f : ex2(__fsub_rn(m, M)); }
@@ -324,7 +324,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
   if (tid == 128) {
     for (int i = 0; i < RING; ++i) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 4); }
     for (int i = 0; i < 2; ++i) { mbar_init(&sm.q_full[i], 1); mbar_init(&sm.q_empty[i], 4); sm.bad[i] = 0; }
-    sm.dead = 0;
+    sm.wait = WaitState{0, 0};
     fence_mbar_init();
   }
   pdl_wait();
@@ -386,7 +386,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
     int e = 0, uq = 0;
     auto load = [&](const CUtensorMap* map, int row) {
       const int st = e % RING;
-      if (!warp_wait(&sm.dead, &sm.empty[st], ((e / RING) & 1) ^ 1, a.err)) return;
+      if (!warp_wait(&sm.wait, &sm.empty[st], ((e / RING) & 1) ^ 1, a.err)) return;
       if (lane == 0) mbar_expect_tx(&sm.full[st], kTile * Dh * 2);
       __syncwarp();
       const int r = __shfl_sync(0xFFFFFFFFu, row, min(part, parts - 1));
@@ -403,7 +403,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       if (j < x.k_end) row = part_row(x, j);
     }
     bool head = true;
-    while (u < units && !*reinterpret_cast<volatile int*>(&sm.dead)) {
+    while (u < units && !given_up(&sm.wait)) {
       // the tile after this one, its table entries on their way while this one's copies are issued
       DecodeUnit xn = x;
       int un = u, jn = j < x.k_end ? next_tile(x, j + kTile) : x.k_end;
@@ -421,7 +421,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       }
       if (head) {  // the unit's query rows (their place may still be in use: behind the first copies)
         const int st = uq % QS, rows = min(8 * NT, R - x.row0);
-        if (!warp_wait(&sm.dead, &sm.q_empty[st], ((uq / QS) & 1) ^ 1, a.err)) break;
+        if (!warp_wait(&sm.wait, &sm.q_empty[st], ((uq / QS) & 1) ^ 1, a.err)) break;
         if (lane == 0) mbar_expect_tx(&sm.q_full[st], rows * Dh * 2);
         __syncwarp();
         if (lane < rows) {
@@ -437,7 +437,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       j = jn;
       row = row_n;
     }
-    if (*reinterpret_cast<volatile int*>(&sm.dead)) {  // copies in flight end before the CTA does
+    if (given_up(&sm.wait)) {  // copies in flight end before the CTA does
       for (int i = max(0, e - RING); i < e; ++i) mbar_wait_bounded(&sm.full[i % RING], (i / RING) & 1, a.err, 1u << 22);
       for (int i = max(0, uq - QS); i < uq; ++i) mbar_wait_bounded(&sm.q_full[i % QS], (i / QS) & 1, a.err, 1u << 22);
     }
@@ -467,11 +467,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[y][t][i] = 0.0f;
     }
-    warp_wait(&sm.dead, &sm.q_full[uq % QS], (uq / QS) & 1, a.err);
+    warp_wait(&sm.wait, &sm.q_full[uq % QS], (uq / QS) & 1, a.err);
     const uint32_t qbase = smem_u32(sm.q[uq % QS]) + (lane & 7) * (Dh + 8) * 2 + (lane >> 3) * 16;
     for (int j = next_tile(x, x.k_begin); j < x.k_end; j = next_tile(x, j + kTile)) {
       const int sk = e % RING, sv = (e + 1) % RING;
-      warp_wait(&sm.dead, &sm.full[sk], (e / RING) & 1, a.err);
+      warp_wait(&sm.wait, &sm.full[sk], (e / RING) & 1, a.err);
       float s[KG][NT][4];
 #pragma unroll
       for (int g = 0; g < KG; ++g)
@@ -552,7 +552,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
           }
           l[t][i] = __fmaf_rn(l[t][i], alpha[t][i], sum);
         }
-      warp_wait(&sm.dead, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
+      warp_wait(&sm.wait, &sm.full[sv], ((e + 1) / RING) & 1, a.err);
       if (j + kTile > x.len || (a.vis.window != 0 && j < x.lo)) {
         // values that no row sees may be anything, and their weight 0 has to stay 0: cleared
         uint8_t* v = reinterpret_cast<uint8_t*>(sm.kv[sv]);
@@ -647,6 +647,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         float* dst = (FUSED ? reinterpret_cast<float*>(sm.kv) : a.ws_o) + at * Dh;
         for (int i = 0; i < Dh / 32; ++i) dst[lane * (Dh / 32) + i] = oo[i];
         if (lane == 0) (FUSED ? sm.ml : a.ws_ml)[at] = make_float2(mm, ll);
+        sign_of_life(&sm.wait);
       }
     }
   }

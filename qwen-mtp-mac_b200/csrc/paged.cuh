@@ -89,58 +89,107 @@ __device__ __forceinline__ long long cache_row(const PagedView& c, int b, int kh
   return ((pg * c.nkv + kh) << c.page_log) + (j & ((1 << c.page_log) - 1));
 }
 
+// N consecutive bf16 values (N 2, 4 or 8, aligned to their size), two a word.
+template <int N>
+__device__ __forceinline__ void load_dims(uint32_t (&w)[N / 2], const uint16_t* p) {
+  if constexpr (N == 8) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 4) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
 // One query row over the keys [j0, j1) of its sequence that it sees, by one warp: lane l owns dims
 // [l * Dh / 32, (l + 1) * Dh / 32).  One pass with the running maximum m (base 2), sum l and numerator o of
 // the softmax, which the caller starts at (-inf, 0, 0).  Only rows that are seen are read, so nothing
-// behind the mask can reach o.
+// behind the mask can reach o.  The rows of eight keys are on their way at once.
 template <int Dh>
 __device__ __noinline__ void attend_row_strict(const PagedView c, const uint16_t* __restrict__ qrow, int b, int kh,
                                                int p, int j0, int j1, Visible vis, float scale2, unsigned* err,
                                                float& m, float& l, float (&o)[Dh / 32]) {
-  constexpr int N = Dh / 32;
-  const int lane = threadIdx.x & 31;
+  constexpr int N = Dh / 32, AHEAD = 8;
+  const int lane = threadIdx.x & 31, end = min(j1, p + 1);
   float q[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) q[e] = bf2f(qrow[lane * N + e]);
-  for (int j = j0; j < j1 && j <= p; ++j) {
-    if (!vis(p, j)) continue;
-    const long long r = cache_row(c, b, kh, j, err);
-    float s = 0.0f;
-    if (r >= 0)
+  for (int j = j0; j < end; j += AHEAD) {
+    const bool sees = lane < AHEAD && j + lane < end && vis(p, j + lane);
+    const unsigned seen = __ballot_sync(0xFFFFFFFFu, sees);
+    if (seen == 0) continue;
+    const long long row = sees ? cache_row(c, b, kh, j + lane, err) : -1;
+    uint32_t k[AHEAD][N / 2], v[AHEAD][N / 2];
 #pragma unroll
-      for (int e = 0; e < N; ++e) s = __fmaf_rn(q[e], bf2f(c.k[r * Dh + lane * N + e]), s);
-    s = __fmul_rn(warp_sum(s), scale2);
-    const float mn = fmaxf(m, s);
-    const float safe = mn == -INFINITY ? 0.0f : mn;
-    const float a = exp2f(__fsub_rn(m, safe)), w = exp2f(__fsub_rn(s, safe));
-    l = __fmaf_rn(l, a, w);
+    for (int i = 0; i < AHEAD; ++i) {
+      const long long r = __shfl_sync(0xFFFFFFFFu, row, i);
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = r >= 0 ? bf2f(c.v[r * Dh + lane * N + e]) : 0.0f;
-      o[e] = __fmaf_rn(w, x, __fmul_rn(o[e], a));
+      for (int e = 0; e < N / 2; ++e) k[i][e] = v[i][e] = 0;
+      if (r >= 0) {
+        load_dims<N>(k[i], c.k + r * Dh + lane * N);
+        load_dims<N>(v[i], c.v + r * Dh + lane * N);
+      }
     }
-    m = mn;
+    float s[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      s[i] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[i] = __fmaf_rn(q[e], e & 1 ? bfhi(k[i][e / 2]) : bflo(k[i][e / 2]), s[i]);
+      s[i] = __fmul_rn(warp_sum(s[i]), scale2);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (!(seen >> i & 1)) continue;
+      const float mn = fmaxf(m, s[i]);
+      const float safe = mn == -INFINITY ? 0.0f : mn;
+      const float a = exp2f(__fsub_rn(m, safe)), w = exp2f(__fsub_rn(s[i], safe));
+      l = __fmaf_rn(l, a, w);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        o[e] = __fmaf_rn(w, e & 1 ? bfhi(v[i][e / 2]) : bflo(v[i][e / 2]), __fmul_rn(o[e], a));
+      m = mn;
+    }
   }
 }
 
-// A bounded barrier wait.  Once one has run out (`dead`, in shared memory; the error word tells), the CTA's other
-// waits give up soon too.  False: gave up.
-__device__ __forceinline__ bool bar_wait_slow(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
+// What a CTA's barrier waits share, in shared memory.  A wait gives up after 2^20 polls without a sign of life from a warp
+// that is at long work of its own (rows computed by the definition); the others then give up soon too.
+struct WaitState {
+  int dead;   // a wait has run out (the error word tells)
+  int alive;  // counts the signs
+};
+__device__ __forceinline__ bool given_up(const WaitState* w) { return *reinterpret_cast<const volatile int*>(&w->dead) != 0; }
+__device__ __forceinline__ void sign_of_life(WaitState* w) {
+  if ((threadIdx.x & 31) == 0) atomicAdd(&w->alive, 1);
+}
+
+// A bounded barrier wait.  False: gave up.
+__device__ __forceinline__ bool bar_wait_slow(WaitState* w, uint64_t* bar, uint32_t parity, unsigned* err) {
+  const volatile int* alive = &w->alive;
+  int last = *alive;
 #pragma unroll 1
-  for (uint32_t it = 0; it < (1u << 20); ++it) {  // seconds
+  for (uint32_t it = 0; it < (1u << 20); ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 63) == 63 && *reinterpret_cast<volatile int*>(dead)) return false;
+    if ((it & 63) == 63) {
+      if (given_up(w)) return false;
+      const int now = *alive;
+      if (now != last) it = 0;
+      last = now;
+    }
   }
   atomicOr(err, DEVERR_TIMEOUT);
-  *reinterpret_cast<volatile int*>(dead) = 1;
+  *reinterpret_cast<volatile int*>(&w->dead) = 1;
   return false;
 }
-__device__ __forceinline__ bool bar_wait(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
-  return mbar_try_wait(bar, parity) || bar_wait_slow(dead, bar, parity, err);
+__device__ __forceinline__ bool bar_wait(WaitState* w, uint64_t* bar, uint32_t parity, unsigned* err) {
+  return mbar_try_wait(bar, parity) || bar_wait_slow(w, bar, parity, err);
 }
 // By every lane of a warp, which is converged afterwards.
-__device__ __forceinline__ bool warp_wait(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
-  return __all_sync(0xFFFFFFFFu, bar_wait(dead, bar, parity, err));
+__device__ __forceinline__ bool warp_wait(WaitState* w, uint64_t* bar, uint32_t parity, unsigned* err) {
+  return __all_sync(0xFFFFFFFFu, bar_wait(w, bar, parity, err));
 }
 
 __device__ __forceinline__ void prefetch_tensormap(const void* tmap) {

@@ -76,7 +76,7 @@ struct PromptBars {
   alignas(16) uint4 next[1];
   PromptItem item[2];
   uint32_t tmem;
-  int dead;  // a wait ran out: every later wait returns at once
+  WaitState wait;
 };
 
 // What an item's key tiles are, from its place.
@@ -218,8 +218,8 @@ __device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // warp_wait / bar_wait for what another CTA of the cluster released.
-__device__ __forceinline__ bool bar_wait_cluster(int* dead, uint64_t* bar, uint32_t parity, unsigned* err) {
-  const bool ok = bar_wait(dead, bar, parity, err);
+__device__ __forceinline__ bool bar_wait_cluster(WaitState* w, uint64_t* bar, uint32_t parity, unsigned* err) {
+  const bool ok = bar_wait(w, bar, parity, err);
   asm volatile("fence.acq_rel.cluster;" ::: "memory");
   return ok;
 }
@@ -270,6 +270,123 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(x));
   return x != 0;
 }
+// A sign of life to the warps that wait in this CTA and, PAIR, in the other.
+template <bool PAIR>
+__device__ __forceinline__ void sign_of_life_all(WaitState* w) {
+  if (!PAIR) return sign_of_life(w);
+  if ((threadIdx.x & 31) < 2)
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], 1;" ::"r"(in_cta(&w->alive, threadIdx.x & 31)) : "memory");
+}
+
+// Settles the rows `todo` of a softmax warp (bit = lane = row) whose O holds infinities or NaN: from values that the row
+// sees, as 0 * inf from values in its tiles that it does not see, or from a sum beyond fp32.  What is finite in O is right.
+// Where the row sees an infinity or NaN in a dim, that is the dim's result: found by one pass over the values that the
+// warp's rows see, lane l looking after dims [l Dh / 32, (l + 1) Dh / 32) of all rows, which ends once every such dim of O
+// is NaN.  Rows with a dim that no seen value explains are computed again by the definition, reading seen keys only: few,
+// next to a value that is not finite and not theirs.  16384 tokens, 8 / 2 heads of 256 (0.67 ms): an infinity near the start
+// 15 ms, every value NaN 1.2, a last token of NaN 180 (127 tokens by the definition).
+template <int Dh>
+__device__ __noinline__ void settle_rows(const PagedView c, const PromptArgs a, const PromptItem x, WaitState* wait,
+                                         int tile0, uint32_t t_o, unsigned todo) {
+  constexpr int N = Dh / 32, AHEAD = 8;
+  constexpr bool PAIR = PromptCfg<Dh>::PAIR;
+  const int lane = threadIdx.x & 31, row0 = threadIdx.x & 96;
+  const PromptTiles ts(x, a, PromptCfg<Dh>::NQ);
+  const bool mine = todo >> lane & 1;
+  const int p = x.len - x.n + tile0 + (row0 + lane) / a.G;
+  // per dim of this lane, a bit for each row: not finite in O; NaN, inf, -inf among the values seen
+  unsigned odd[N], nans[N], pos[N], neg[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) odd[e] = nans[e] = pos[e] = neg[e] = 0;
+#pragma unroll 1
+  for (int d = 0; d < Dh; d += 32) {
+    float o[32];
+    tmem_ld32_nowait(t_o + d, o);
+    tmem_ld32_ready(o);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const unsigned rows = __ballot_sync(0xFFFFFFFFu, !isfinite(o[i])) & todo;
+      if (lane == (d + i) / N) odd[i % N] = rows;
+    }
+  }
+#pragma unroll 1
+  for (int t = 0; t < ts.nt; ++t) {
+    const int end = min(ts.key(t) + kKeys, ts.p_last + 1);
+#pragma unroll 1
+    for (int j = ts.key(t); j < end; j += AHEAD) {
+      unsigned seen_by[AHEAD], need = 0;
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        seen_by[i] = __ballot_sync(0xFFFFFFFFu, mine && j + i < end && a.vis(p, j + i));
+        need |= unsigned(seen_by[i] != 0) << i;
+      }
+      if (need == 0) continue;
+      const long long row = lane < AHEAD && (need >> lane & 1) ? cache_row(c, x.b, x.kh, j + lane, a.err) : -1;
+      uint32_t v[AHEAD][N / 2];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const long long r = __shfl_sync(0xFFFFFFFFu, row, i);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) v[i][e] = 0;
+        if (r >= 0) load_dims<N>(v[i], c.v + r * Dh + lane * N);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const uint32_t bits = e & 1 ? v[i][e / 2] >> 16 : v[i][e / 2] & 0xFFFFu;
+          if ((bits & 0x7F80u) != 0x7F80u) continue;
+          if (bits & 0x7Fu)
+            nans[e] |= seen_by[i];
+          else if (bits & 0x8000u)
+            neg[e] |= seen_by[i];
+          else
+            pos[e] |= seen_by[i];
+        }
+    }
+    sign_of_life_all<PAIR>(wait);
+    unsigned open = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) open |= odd[e] & ~(nans[e] | (pos[e] & neg[e]));
+    if (!__any_sync(0xFFFFFFFFu, open != 0)) break;
+  }
+  unsigned again = 0;  // rows to compute by the definition
+#pragma unroll
+  for (int e = 0; e < N; ++e) again |= odd[e] & ~(nans[e] | pos[e] | neg[e]);
+  again = __reduce_or_sync(0xFFFFFFFFu, again);
+  while (todo) {
+    const int src = __ffs(todo) - 1;
+    todo &= todo - 1;
+    const int ti = tile0 + (row0 + src) / a.G, h = x.kh * a.G + (row0 + src) % a.G, pr = x.len - x.n + ti;
+    const long long tr = x.c0 + ti, orow = (tr * a.nq + h) * Dh;
+    const bool redo = again >> src & 1;
+    float m = -INFINITY, l = 0.0f, o[N] = {};
+    if (redo)
+      for (int t = 0; t < ts.nt; ++t) {
+        attend_row_strict<Dh>(c, a.q + tr * a.q_ld + (long long)h * Dh, x.b, x.kh, pr, ts.key(t), ts.key(t) + kKeys, a.vis,
+                              a.scale2, a.err, m, l, o);
+        sign_of_life_all<PAIR>(wait);
+      }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool up = pos[e] >> src & 1, down = neg[e] >> src & 1, known = up || down || (nans[e] >> src & 1);
+      if (!known && !redo) continue;
+      const int d = lane * N + e;
+      float y = up ? INFINITY : -INFINITY;
+      if ((nans[e] >> src & 1) || (up && down)) y = __int_as_float(0x7FFFFFFF);
+      if (a.splits > 1) {
+        a.ws_o[(long long)x.split * a.T * a.nq * Dh + orow + d] = known ? y : o[e];
+        continue;
+      }
+      if (!known) y = pr < 0 ? 0.0f : __fdiv_rn(o[e], l);
+      if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[tr * a.gate_ld + h * a.gate_hs + d])));
+      a.out[orow + d] = f2bf(y);
+    }
+    if (redo && a.splits > 1 && lane == 0) a.ws_ml[((long long)x.split * a.T + tr) * a.nq + h] = make_float2(m, l);
+  }
+  __syncwarp();
+}
+
 template <int Dh>
 __global__ void __launch_bounds__(PromptCfg<Dh>::threads, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -317,7 +434,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       mbar_init(&bars->item_full[i], 1);
       mbar_init(&bars->item_empty[i], 10);  // a pair: 4 + 1 warps each; else 8 + 2
     }
-    bars->dead = 0;
+    bars->wait = WaitState{0, 0};
     fence_mbar_init();
   }
   pdl_wait();
@@ -387,12 +504,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       }
       auto take_over = [&] {  // the block that the request of this round has got, or -1
         int next = -1;
-        if (a.takes_over && bar_wait(&bars->dead, &bars->next_full, asked & 1, a.err)) next = next_block(bars->next);
+        if (a.takes_over && bar_wait(&bars->wait, &bars->next_full, asked & 1, a.err)) next = next_block(bars->next);
         ++asked;
         return __shfl_sync(0xFFFFFFFFu, next, 0);
       };
       auto hand_out = [&](const PromptItem& y, int at) {
-        const bool ok = warp_wait(&bars->dead, &bars->item_empty[at & 1], ((at >> 1) & 1) ^ 1, a.err);
+        const bool ok = warp_wait(&bars->wait, &bars->item_empty[at & 1], ((at >> 1) & 1) ^ 1, a.err);
         if (lane == 0) {
           bars->item[at & 1] = y;
           mbar_arrive(&bars->item_full[at & 1]);
@@ -421,7 +538,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       if (rank == 0 || (own && x.b >= 0)) {
         ok = hand_out(x, i);
       } else {  // the second CTA finds the block's own item itself and is told of the others
-        ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(&bars->dead, &bars->item_full[i & 1], (i >> 1) & 1, a.err));
+        ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(&bars->wait, &bars->item_full[i & 1], (i >> 1) & 1, a.err));
         if (!ok) break;
         x = bars->item[i & 1];
         __syncwarp();
@@ -439,11 +556,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         };
         auto load = [&](const CUtensorMap* map, int pos, bool is_v, int row, bool tail) {
           const int e = e0 + pos, st = e % NS;
-          if (!warp_wait(&bars->dead, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err)) return;
+          if (!warp_wait(&bars->wait, &bars->empty[st], ((e / NS) & 1) ^ 1, a.err)) return;
           // PAIR: the copies of both CTAs count on the first one's barrier; those of a V tile in which the sequence ends
           // on their own CTA's, whose softmax warps clear it and answer with their weights.  The barrier is free again
           // once the item before (number loads - 2) is done: its last product took every warp's weights.
-          if (PAIR && tail && loads > 1 && !warp_wait(&bars->dead, &bars->done[0], loads & 1, a.err)) return;
+          if (PAIR && tail && loads > 1 && !warp_wait(&bars->wait, &bars->done[0], loads & 1, a.err)) return;
           if (lane == 0) {
             if (PAIR && tail) mbar_expect_tx(&bars->tail, Cfg::entry);
             if (PAIR && tail && rank == 0) mbar_arrive(&bars->full[st]);
@@ -467,7 +584,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           if (tail) ++tails;
         };
         auto load_q = [&] {
-          if (!warp_wait(&bars->dead, &bars->q_empty, (loads & 1) ^ 1, a.err)) return;
+          if (!warp_wait(&bars->wait, &bars->q_empty, (loads & 1) ^ 1, a.err)) return;
           if (lane == 0 && rank == 0) mbar_expect_tx(&bars->q_full, uint32_t(PAIR ? 2 : ts.chains) * a.G * a.tpt * Dh * 2);
           __syncwarp();
           if (lane < ts.chains * CB) {
@@ -512,7 +629,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       }
       u = next / (PAIR ? 2 : 1);
     }
-    if (*reinterpret_cast<volatile int*>(&bars->dead)) {  // copies in flight end before the CTA does
+    if (given_up(&bars->wait)) {  // copies in flight end before the CTA does
       if (a.takes_over && asked > 0) mbar_wait_bounded(&bars->next_full, (asked - 1) & 1, a.err, 1u << 22);
       if (tails > 0) mbar_wait_bounded(&bars->tail, (tails - 1) & 1, a.err, 1u << 22);
       if (loads > 0 && rank == 0) mbar_wait_bounded(&bars->q_full, (loads - 1) & 1, a.err, 1u << 22);
@@ -529,7 +646,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       const uint64_t qd = desc_sw128(smem_u32(s_q + w * Cfg::q_bytes), 16, 1024);
       int e0 = 0, work = 0, g = 0, finished = 0;  // g: score tiles so far
       for (int items = 0;; ++items) {
-        if (!bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)) break;
+        if (!bar_wait(&bars->wait, &bars->item_full[items & 1], (items >> 1) & 1, a.err)) break;
         const PromptItem x = bars->item[items & 1];
         mbar_arrive(&bars->item_empty[items & 1]);
         if (x.b < 0) break;
@@ -539,7 +656,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           auto used = [&](uint64_t* bar) { mma_commit<PAIR>(bar); };  // an entry is free when both row tiles have used it
           auto scores = [&](int j) {  // S = Q K^T of score tile j
             const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, e = e0 + pos_k(t), st = e % NS;
-            if (r0 == 0) bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+            if (r0 == 0) bar_wait(&bars->wait, &bars->full[st], (e / NS) & 1, a.err);
             tc_fence_after();
             const uint64_t kd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + r0 * 128, 16, 1024);
 #pragma unroll
@@ -552,10 +669,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           };
           auto values = [&](int j) {  // O += P V of score tile j
             const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, e = e0 + pos_v(t, nt), st = e % NS;
-            if (r0 == 0) bar_wait(&bars->dead, &bars->full[st], (e / NS) & 1, a.err);
+            if (r0 == 0) bar_wait(&bars->wait, &bars->full[st], (e / NS) & 1, a.err);
 #pragma unroll
             for (int hf = 0; hf < SUB / 64; ++hf) {  // 64 keys, as the softmax hands them over
-              bar_wait(&bars->dead, &bars->p_full[w][buf][hf], ((g + j) >> 1) & 1, a.err);
+              bar_wait(&bars->wait, &bars->p_full[w][buf][hf], ((g + j) >> 1) & 1, a.err);
               tc_fence_after();
               const uint64_t vd = desc_sw128(smem_u32(s_ring + st * Cfg::entry) + (r0 + hf * 64) * 128, kKeys * 128, 1024);
 #pragma unroll
@@ -565,7 +682,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
             mma_commit<PAIR>(j + 1 < subs ? &bars->pv[w] : &bars->done[w]);
             if (j % NQ == NQ - 1 || j + 1 == subs) used(&bars->empty[st]);
           };
-          bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
+          bar_wait(&bars->wait, &bars->q_full, work & 1, a.err);
           // S0 S1 | O0 S2 | O1 S3 ...: the next scores are always under way while the softmax works
           for (int j = 0; j < min(2, subs); ++j) scores(j);
           for (int j = 0; j < subs; ++j) {
@@ -578,10 +695,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           // A row tile without tokens: its thread follows the item's barriers all the same.  A wait by parity is only right
           // for the phase after the last one that its thread has seen: behind a skipped item it could pass while the item's own
           // copies were under way, and the next one's products read tiles that were not there.
-          bar_wait(&bars->dead, &bars->q_full, work & 1, a.err);
+          bar_wait(&bars->wait, &bars->q_full, work & 1, a.err);
           mbar_arrive(&bars->q_empty);
           for (int e = e0; e < e0 + 2 * nt; ++e) {
-            bar_wait(&bars->dead, &bars->full[e % NS], (e / NS) & 1, a.err);
+            bar_wait(&bars->wait, &bars->full[e % NS], (e / NS) & 1, a.err);
             mbar_arrive(&bars->empty[e % NS]);
           }
         }
@@ -601,8 +718,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
     int e0 = 0, tails = 0;             // ring entries of the items so far, V tiles cleared
     int turns = 0;
     for (int items = 0;; ++items) {
-      if (!__all_sync(0xFFFFFFFFu, PAIR ? bar_wait_cluster(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)
-                                        : bar_wait(&bars->dead, &bars->item_full[items & 1], (items >> 1) & 1, a.err)))
+      if (!__all_sync(0xFFFFFFFFu, PAIR ? bar_wait_cluster(&bars->wait, &bars->item_full[items & 1], (items >> 1) & 1, a.err)
+                                        : bar_wait(&bars->wait, &bars->item_full[items & 1], (items >> 1) & 1, a.err)))
         break;
       const PromptItem x = bars->item[items & 1];
       __syncwarp();
@@ -626,7 +743,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       for (int j = 0; j < ts.subs; ++j) {
         const int buf = (g + j) & 1, t = j / NQ, r0 = (j - t * NQ) * SUB, j0 = ts.key(t) + r0;
         const uint32_t t_s = tmem + lane_base + 256 + (2 * w + buf) * SUB;
-        warp_wait(&bars->dead, &bars->s_full[w][buf], ((g + j) >> 1) & 1, a.err);
+        warp_wait(&bars->wait, &bars->s_full[w][buf], ((g + j) >> 1) & 1, a.err);
         tc_fence_after();
         float s[SUB];
 #pragma unroll
@@ -635,7 +752,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           // The sequence ends in this tile: the values behind its end may be anything, and their weight 0 has to stay
           // 0.  They are cleared before the weights are handed over.
           const int e = e_item + pos_v(t, nt), st = e % NS;
-          warp_wait(&bars->dead, PAIR ? &bars->tail : &bars->full[st], PAIR ? tails & 1 : (e / NS) & 1, a.err);
+          warp_wait(&bars->wait, PAIR ? &bars->tail : &bars->full[st], PAIR ? tails & 1 : (e / NS) & 1, a.err);
           ++tails;
           for (int i = r; i < Cfg::entry / 16 / kKeys * SUB; i += 128) {
             const int row = (i >> 3) % SUB, cb = (i >> 3) / SUB;
@@ -666,7 +783,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
           const float alpha = mn == -INFINITY ? 1.0f : ex2(__fsub_rn(m, mn));
           m = mn;
           l = __fmul_rn(l, alpha);
-          warp_wait(&bars->dead, &bars->pv[w], (pvs + j - 1) & 1, a.err);
+          warp_wait(&bars->wait, &bars->pv[w], (pvs + j - 1) & 1, a.err);
           tc_fence_after();
 #pragma unroll 1
           for (int d = 0; d < Dh; d += 32) {
@@ -683,7 +800,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         const uint64_t scale2 = f2_pack(a.scale2, a.scale2), neg2 = f2_pack(neg, neg);
         uint64_t sum[2] = {0, 0};
         if (NQ == 2 && ts.chains == 2) {  // the k-th time: row tile 1 behind tile 0's k-th, tile 0 behind tile 1's (k - 1)-th
-          if (w == 1 || turns > 0) warp_wait(&bars->dead, &bars->turn[w][warp & 3], (turns - 1 + w) & 1, a.err);
+          if (w == 1 || turns > 0) warp_wait(&bars->wait, &bars->turn[w][warp & 3], (turns - 1 + w) & 1, a.err);
           ++turns;
         }
 #pragma unroll
@@ -739,11 +856,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
       g += ts.subs;
       if (nt > 0) {
         pvs += ts.subs - 1;
-        warp_wait(&bars->dead, &bars->done[w], finished & 1, a.err);
+        warp_wait(&bars->wait, &bars->done[w], finished & 1, a.err);
         ++finished;
         tc_fence_after();
       }
-      // O / l, gate, store; a row with an infinity or NaN is settled by the definition afterwards
+      // O / l, gate, store; a row with an infinity or NaN in O is settled afterwards
       const long long orow = (row * a.nq + h) * Dh;
       const float inv = p < 0 ? 0.0f : __fdiv_rn(1.0f, l);  // l = 0 at p >= 0: every score seen is -inf, 0 / 0
       float* part = a.ws_o + (long long)x.split * a.T * a.nq * Dh + orow;
@@ -798,32 +915,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constan
         __syncwarp();
       }
       const bool odd = !(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
-      tc_fence_before();
       if (valid && a.splits > 1) a.ws_ml[((long long)x.split * a.T + row) * a.nq + h] = make_float2(m, l);
-      unsigned todo = __ballot_sync(0xFFFFFFFFu, odd && valid);
-      while (todo) {
-        const int src = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const int rr = (tid & 127 & ~31) + src, ti = tile0 + rr / a.G, hh = x.kh * a.G + rr % a.G;
-        const long long tr = x.c0 + ti;
-        float mm = -INFINITY, ll = 0.0f, oo[Dh / 32] = {};
-        for (int t = 0; t < nt; ++t)
-          attend_row_strict<Dh>(c, a.q + tr * a.q_ld + (long long)hh * Dh, x.b, x.kh, x.len - x.n + ti, ts.key(t),
-                                ts.key(t) + kKeys, a.vis, a.scale2, a.err, mm, ll, oo);
-        __syncwarp();
-        for (int e = 0; e < Dh / 32; ++e) {
-          const int d = lane * (Dh / 32) + e;
-          const long long at = (tr * a.nq + hh) * Dh + d;
-          if (a.splits > 1) {
-            a.ws_o[(long long)x.split * a.T * a.nq * Dh + at] = oo[e];
-          } else {
-            float y = x.len - x.n + ti < 0 ? 0.0f : __fdiv_rn(oo[e], ll);  // nothing seen: zeros
-            if (a.gate) y = __fmul_rn(y, sigmoid_f32(bf2f(a.gate[tr * a.gate_ld + hh * a.gate_hs + d])));
-            a.out[at] = f2bf(y);
-          }
-        }
-        if (a.splits > 1 && lane == 0) a.ws_ml[((long long)x.split * a.T + tr) * a.nq + hh] = make_float2(mm, ll);
-      }
+      // a sum l that is NaN makes the whole row NaN, which it is; one of 0 leaves zeros or NaN, except behind NaN in O
+      const unsigned todo =
+          __ballot_sync(0xFFFFFFFFu, odd && valid && l == l && (l != 0.0f || (p < 0 && a.splits == 1)));
+      if (todo) settle_rows<Dh>(c, a, x, &bars->wait, tile0, t_o, todo);
+      tc_fence_before();
     }
   }
   tc_fence_before();

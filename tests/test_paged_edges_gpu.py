@@ -173,3 +173,83 @@ def test_prompt_lone_and_paired_row_tiles_in_turn(nq, nkv, dh, dev):
         wrong[i] = (paged.prompt_attention(*bt.args(), bt.d["cu"]) != alone).any()
     assert device_error() == 0
     assert not wrong.any(), int(wrong.sum())
+def check_classes(out, ref, bt, marks, window=0, sinks=0, gate=None):
+    """out against ref in every (row, dim) whose seen values are finite; in the others the infinity or NaN that the seen
+    marks (sequence, position, dim, value) add up to."""
+    out = out.cpu().view(bt.T, bt.nq, bt.dh)
+    r, kind = 0, torch.zeros(bt.T, bt.dh, dtype=torch.long)  # bits: inf 1, -inf 2, NaN 4
+    for b, (n, length) in enumerate(bt.sizes):
+        for i in range(n):
+            p = length - n + i
+            for mb, j, d, value in marks:
+                if mb == b and j <= p and (not window or p - j < window or j < sinks):
+                    kind[r, d] |= 1 if value == float("inf") else 2 if value == float("-inf") else 4
+            r += 1
+    kind = kind[:, None].expand(-1, bt.nq, -1)
+    assert (out[kind == 1] == float("inf")).all() and (out[kind == 2] == float("-inf")).all()
+    assert torch.isnan(out[kind >= 3]).all()
+    rows = (kind == 0).reshape(bt.T, -1)
+    check(out.reshape(bt.T, -1)[rows], (ref[0][rows], ref[1][rows]))
+
+
+@pytest.mark.parametrize("table_extra", [0, 200])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+@pytest.mark.parametrize("dh,nq,nkv", [(256, 8, 2), (128, 6, 2), (64, 3, 3)])
+def test_prompt_values_that_are_not_finite(dh, nq, nkv, window, sinks, table_extra, dev):
+    """Infinities and NaN in values that some rows of a chunk see and others do not: single dims and whole rows, at the
+    start, inside and at the end of the sequences, opposite ones in one dim, keys split over blocks and not."""
+    from qmtp import paged
+
+    inf, nan = float("inf"), float("nan")
+    bt = Batch([(150, 420), (70, 70), (5, 2), (33, 260)], nq, nkv, dh, 16, seed=dh + window, table_extra=table_extra)
+    ref = attention_ref(bt, window, sinks)
+    marks = [(0, 0, 3, inf), (0, 300, 7, -inf), (0, 330, 7, inf), (0, 419, 9, nan), (1, 2, 1, -inf), (2, 1, 4, inf),
+             (3, 100, 11, inf), (3, 200, 12, nan), (3, 259, 13, -inf)]
+    marks += [(1, 40, d, nan) for d in range(dh)]
+    for b, j, d, value in marks:
+        pg, sl = bt.rows(b, j)
+        bt.v[pg, :, sl, d] = value
+    bt.put(dev)
+    call = lambda: paged.prompt_attention(*bt.args(), bt.d["cu"], gate=bt.d["gate"][:, :, 1], window=window, sinks=sinks)
+    out = call()
+    assert device_error() == 0
+    check_classes(out, ref, bt, marks, window, sinks)
+    assert torch.equal(call().view(torch.int16), out.view(torch.int16))
+
+
+@pytest.mark.parametrize("dh,nq,nkv", [(256, 8, 2), (128, 8, 2), (64, 4, 4)])
+def test_prompt_long_sequence_with_values_that_are_not_finite(dh, nq, nkv, dev):
+    """16384 tokens with an infinite value early, and with a token late whose value is NaN: no wait runs out while rows are
+    computed again, and what does not see them stays what it is without them."""
+    from qmtp import paged
+
+    T = 16384
+    g = torch.Generator(device=dev).manual_seed(dh)
+    rnd = lambda *s: torch.randn(s, generator=g, device=dev).to(BF16)
+    cache = paged.PagedCache(rnd(T // 64, nkv, 64, dh), rnd(T // 64, nkv, 64, dh))
+    q = rnd(T, nq, dh)
+    table = torch.arange(T // 64, dtype=torch.int32, device=dev)[None]
+    lens, cu = torch.tensor([T], dtype=torch.int32, device=dev), torch.tensor([0, T], dtype=torch.int32, device=dev)
+    call = lambda c: paged.prompt_attention(q, c, table, lens, cu).view(T, nq, dh)
+    clean = call(cache)
+    # each of two results is this far from the exact one: its rounding, the weights', and the scores' error in the exponent
+    # (|q . k| <= |q| |k|), against A = sum p |v|, which is itself a result within 2^-6 of the exact one
+    A = call(paged.PagedCache(cache.k, cache.v.abs())).double() * (1 + 2.0 ** -6)
+    e = dh ** -0.5 * dh * 2.0 ** -22 * float(q.float().norm(dim=-1).max() * cache.k.float().norm(dim=-1).max()) + 2.0 ** -20
+    near = lambda a, rows: ((a[rows].double() - clean[rows].double()).abs()
+                            <= 2 * (2.0 ** -8 * (1 + 2.0 ** -7) * clean[rows].double().abs() + (2.0 ** -8 + 2 * e) * A[rows])).all()
+    held = cache.v.clone()
+    cache.v[1, :, 36, 5] = float("inf")  # position 100
+    out = call(cache)
+    assert device_error() == 0
+    assert (out[100:, :, 5] == float("inf")).all() and near(out, slice(0, 100))
+    rest = torch.arange(dh, device=dev) != 5
+    assert torch.equal(out[100:, :, rest], clean[100:, :, rest])
+    cache.v.copy_(held)
+    cache.v[16000 // 64, :, 0] = float("nan")
+    out = call(cache)
+    assert device_error() == 0
+    assert torch.isnan(out[16000:]).all() and near(out, slice(0, 16000))
+    assert torch.equal(out[:15800], clean[:15800])
+    cache.v.fill_(float("nan"))
+    assert torch.isnan(call(cache)).all() and device_error() == 0
