@@ -666,7 +666,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
       // class k: slab number k of the first ones (few calls have any), and the one of the others with that residue
       float m1[16], l1[16];
       int part_of[16];
-      unsigned absent = 0;
       float M = kNone;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -674,11 +673,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
         part_of[k] = pt < n_parts ? pt : 0;
         m1[k] = ld_dsmem(mlp, part_of[k]);
         l1[k] = ld_dsmem(mlp + 1, part_of[k]);
-        if (pt >= n_parts) {  // a class without a slab adds nothing, whatever the slab read in its place holds
-          m1[k] = kNone;
-          l1[k] = 0.0f;
-          absent |= 1u << k;
-        }
+        if (pt >= n_parts) m1[k] = kNone;
         M = fmaxf(M, m1[k]);
       }
       for (int k = 0; k < mine_slabs.first; ++k) M = fmaxf(M, ld_dsmem(mlp, k));
@@ -689,7 +684,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           v[k] = ld_dsmem_v4(op, part_of[k0 + k]);
-          if (absent >> (k0 + k) & 1) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);  // 0 times an infinity would be NaN
+          // a class without a slab adds nothing, whatever the slab read in its place holds: 0 times an infinity would be NaN
+          if (mine_slabs.first + ((k0 + k - mine_slabs.from) & 15) >= n_parts) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
