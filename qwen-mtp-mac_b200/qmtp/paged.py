@@ -195,9 +195,16 @@ def _attention_args(q, cache: PagedCache, gate, scale, window, sinks, out):
 
 
 def _launch(cache, what, fn, workspace, a, c, q, *args):
+    """Workspace and launch, both with the tensors' device as the current one: the launch's form goes by its SMs."""
+    index = cache._index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _launch(cache, what, fn, workspace, a, c, q, *args)
     n = workspace(a, c)
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
-    _call(cache._index, what, fn, a, *args, c, _lib.ptr(ws), n)
+    rc = fn(a, *args, c, _lib.ptr(ws), n, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc, what)
 
 
 def attention(q, cache: PagedCache, table, lens, *, gate=None, scale: float | None = None, window: int = 0,
