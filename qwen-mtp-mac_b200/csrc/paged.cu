@@ -64,14 +64,22 @@ __global__ void __launch_bounds__(256) paged_append_kernel(PagedView c, AppendAr
     b = t / a.S;
     p = seq_len(c, b, a.err) - a.S + (t - b * a.S);
   } else {
-    // sequences that end at or before row t, counted a warp at a time (cu does not decrease)
-    b = 0;
+    // the sequence [cu[b], cu[b + 1]) that holds row t, a warp's worth at a time; offsets that are none hold no row
+    b = p = -1;
+    bool bad = false;
     for (int i = 0; i < c.B; i += 32) {
-      const int k = i + lane;
-      b += __popc(__ballot_sync(0xFFFFFFFFu, k < c.B && a.cu[k + 1] <= t));
+      const int k = i + lane, c0 = k < c.B ? a.cu[k] : 0, c1 = k < c.B ? a.cu[k + 1] : 0;
+      const bool good = c0 >= 0 && c0 <= c1 && c1 <= a.T;
+      bad |= !good;
+      const unsigned hit = __ballot_sync(0xFFFFFFFFu, good && c0 <= t && t < c1);
+      if (hit && b < 0) {
+        b = i + __ffs(hit) - 1;
+        p = t - __shfl_sync(0xFFFFFFFFu, c1, __ffs(hit) - 1);
+      }
     }
-    if (b >= c.B || t < a.cu[b]) return;  // a row of no sequence
-    p = seq_len(c, b, a.err) - a.cu[b + 1] + t;
+    if (bad) atomicOr(a.err, DEVERR_BADARG);
+    if (b < 0) return;  // a row of no sequence
+    p += seq_len(c, b, a.err);
   }
   if (p < 0) return;
   const bool far = a.cos_t != nullptr && p >= a.max_pos;

@@ -46,6 +46,39 @@ def test_append_with_one_norm(nq, nkv, dh, rotary, gated, norm, T, dev):
     assert torch.equal(bt.cache.v.cpu().double(), rv)
 
 
+@pytest.mark.parametrize("spare", [0, 40])
+@pytest.mark.parametrize("at,value", [(2, 3), (2, -1), (2, 30), (3, 31), (3, 2 ** 31 - 1), (0, -1), (1, 2 ** 31 - 1)])
+def test_append_row_offsets_that_are_none(at, value, spare, dev):
+    """Offsets that decrease or leave [0, rows] set the error word; the sequences they bound have no rows, the others keep
+    theirs.  ``spare``: empty sequences before and behind, so that offsets fill more than one step of the search."""
+    from qmtp import paged
+
+    sizes = [(0, 5)] * spare + [(10, 20), (10, 20), (10, 20)] + [(0, 5)] * spare
+    bt = Batch(sizes, 2, 1, 64, 16, seed=at)
+    bt.cu[spare + at] = value
+    want_k, want_v = bt.k.clone(), bt.v.clone()
+    qkv = torch.randn((30, 4 * 64), generator=bt.g).to(BF16)
+    want_q = torch.full((30, 2, 64), 3.0, dtype=BF16)
+    offsets = bt.cu.tolist()
+    holder = {}
+    for b in reversed(range(len(sizes))):  # a row that two hold is the first one's
+        c0, c1 = offsets[b], offsets[b + 1]
+        if 0 <= c0 <= c1 <= 30:
+            holder.update({t: (b, c1) for t in range(c0, c1)})
+    for t, (b, c1) in holder.items():
+        p = int(bt.lens[b]) - c1 + t
+        if p >= 0:
+            pg, sl = bt.rows(b, p)
+            want_k[pg, 0, sl], want_v[pg, 0, sl], want_q[t] = qkv[t, 128:192], qkv[t, 192:], qkv[t, :128].view(2, 64)
+    bt.put(dev)
+    out = torch.full((30, 2, 64), 3.0, dtype=BF16, device=dev)
+    paged.append_qkv(qkv.to(dev), bt.cache, bt.d["table"], bt.d["lens"], bt.d["cu"], n_heads=2, out=out)
+    bad = any(not 0 <= c0 <= c1 <= 30 for c0, c1 in zip(offsets, offsets[1:]))  # 0, 10, 30, 30 are offsets
+    assert device_error() == (2 if bad else 0)
+    assert torch.equal(out.cpu(), want_q)
+    assert torch.equal(bt.cache.k.cpu(), want_k) and torch.equal(bt.cache.v.cpu(), want_v)
+
+
 # ------------------------------------------------------------------------------------ attention
 def set_value(bt, b, pos, dim, value):
     """V of position pos of sequence b, every key head: value at dim."""
