@@ -474,7 +474,7 @@ int qmtp_paged_append(const void* qkv, long long ld, int T, const int* cu, int n
  *   gate  bf16 or NULL: head h of row t at gate + t * gate_ld + h * gate_hs (elements), e.g. the gates
  *         that qmtp_paged_append leaves in qkv
  *   out   bf16 [T, n_q * Dh]
- * scale > 0 and finite; window, sinks >= 0; q, gate, out 16-byte aligned, strides multiples of 8. */
+ * scale > 0, scale * log2(e) finite in fp32; window, sinks >= 0; q, gate, out 16-byte aligned, strides multiples of 8. */
 typedef struct qmtp_paged_args {
   const void* q;
   const void* gate;

@@ -887,7 +887,7 @@ int paged_view(const qmtp_paged_cache* c, PagedView* v) {
 
 int paged_check_args(const qmtp_paged_args* a, const qmtp_paged_cache* c) {
   if (!a || !a->q || !a->out) return QMTP_ERR_ARG;
-  if (!(a->scale > 0.0f) || !std::isfinite(a->scale) || a->window < 0 || a->sinks < 0) return QMTP_ERR_ARG;
+  if (!(a->scale > 0.0f) || !std::isfinite(a->scale * kLog2e) || a->window < 0 || a->sinks < 0) return QMTP_ERR_ARG;
   if (a->T < 1 || a->n_q < 1 || a->n_q > kMaxHeads || a->n_q % c->n_kv) return QMTP_ERR_SHAPE;
   if (a->n_q / c->n_kv > 64) return QMTP_ERR_UNSUPPORTED;
   if (a->q_ld % 8 || (a->q_ld && a->q_ld < (long long)a->n_q * c->Dh)) return QMTP_ERR_SHAPE;

@@ -172,8 +172,8 @@ def _attention_args(q, cache: PagedCache, gate, scale, window, sinks, out):
         _need(False, "window and sinks count tokens")
     if scale is None:
         scale = dh ** -0.5
-    elif not 0 < scale < 3e38:
-        _need(False, "scale is positive and finite")
+    elif not 0 < scale < 2.35e38:
+        _need(False, "scale is positive, and scale * log2(e) finite in fp32")
     if T > _INT_MAX or nq > _INT_MAX:
         _need(False, "q is too large")
     if out is None:
