@@ -439,7 +439,8 @@ int qmtp_moe_dispatch(const void* idx, int T, int S, const void* x, int H, int n
  * tokens of sequence b are its last n_b positions lens[b] - n_b .. lens[b] - 1.  A sequence with
  * lens[b] == 0 is empty.  Bad device-side values never read or write outside the arrays: they set bit 1
  * of the device error word, and a sequence whose length is negative or above table_w * page counts as
- * empty, a row of a page outside [0, pages) is read as zeros and not written. */
+ * empty, a row of a page outside [0, pages) is read as zeros and not written, and a sequence whose row
+ * offsets decrease or leave [0, T] has no rows (rows that two others then hold are either's). */
 typedef struct qmtp_paged_cache {
   void* k;
   void* v;
@@ -455,7 +456,7 @@ typedef struct qmtp_paged_cache {
  *   qkv    bf16 [T, ld]: n_q heads of q (gated: (q, gate) pairs, as qmtp_attn_prep), n_kv of k, n_kv of v
  *   cu     int32 [B + 1] or NULL: rows cu[b] .. cu[b+1] are the new tokens of sequence b, in order; rows
  *          outside [cu[0], cu[B]) belong to no sequence.  NULL: T = B * n, n rows for every sequence
- *   q_w, k_w  bf16 [Dh] norm weights, NULL: no norm;  cos_t, sin_t fp32 [max_pos, rotary / 2], NULL (both):
+ *   q_w, k_w  bf16 [Dh] norm weights, each NULL for no norm;  cos_t, sin_t fp32 [max_pos, rotary / 2], NULL (both):
  *          no rotation; rotary a multiple of 16, 16 .. Dh
  *   q_out  bf16 [T, n_q, Dh].  All arithmetic in fp32, one rounding per output; v is copied.
  * A row of no sequence, or at a negative position (a sequence shorter than its row count), is skipped:
@@ -469,7 +470,9 @@ int qmtp_paged_append(const void* qkv, long long ld, int T, const int* cu, int n
  * (query head h reads key head h / (n_q / n_kv)), and with a gate times sigmoid(gate).  The query at
  * position p sees key j <= p when window == 0, or p - j < window, or j < sinks.  A query that sees no
  * key (an empty sequence, a negative position) gives zeros.  Keys and values a query does not see never
- * reach its output, whatever they hold (infinities and NaN included).
+ * reach its output, whatever they hold (infinities and NaN included); those that it sees do, as in the
+ * formula (every score -inf: 0 / 0 = NaN).  The sums are fp32, their weights relative to the largest:
+ * values whose weighted sum passes 2^128 give infinities.
  *   q     bf16 [T, n_q, Dh], rows q_ld elements apart (0: n_q * Dh)
  *   gate  bf16 or NULL: head h of row t at gate + t * gate_ld + h * gate_hs (elements), e.g. the gates
  *         that qmtp_paged_append leaves in qkv
@@ -488,8 +491,12 @@ typedef struct qmtp_paged_args {
 /* Attention of the newest tokens: T = B * S rows, row b * S + s at position lens[b] - S + s; S <= 8,
  * n_q / n_kv <= 64.  A sequence's keys are cut into slabs at fixed positions, the slabs are computed all
  * over the GPU and joined in order, so a token's result has the same bits whatever B, S, the page size
- * and the other sequences are.  workspace: qmtp_paged_attention_workspace bytes, 16-byte aligned (two
- * calls that may run at the same time need their own). */
+ * and the other sequences are, as long as the sequence's keys and values are finite (rows beside an
+ * infinity or NaN are computed in another order).  workspace: qmtp_paged_attention_workspace bytes,
+ * 16-byte aligned (two calls that may run at the same time need their own).  It goes by what the table can
+ * hold, not by the lengths: B x slabs x T / B x n_q x (Dh + 2) floats, slabs of 512 keys of table_w * page
+ * beyond the first 4096 (64 sequences x 3 tokens of 16 / 4 heads of 256, tables of 131072 tokens: 888 MB),
+ * with a window up to 4096 only those that sinks and window can touch; 0 where short tables run in one launch. */
 size_t qmtp_paged_attention_workspace(const qmtp_paged_args* args, const qmtp_paged_cache* cache);
 int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_paged_cache* cache, void* workspace,
                          size_t ws_bytes, void* stream);
@@ -498,7 +505,9 @@ int qmtp_paged_attention(const qmtp_paged_args* args, const qmtp_paged_cache* ca
  * the last tokens of sequence b, whose keys and values are already in the cache (qmtp_paged_append).
  * Runs on the tensor cores (tcgen05).  Rows of out outside every sequence are left as they were.
  * n_q / n_kv <= 64.  workspace: qmtp_paged_prompt_workspace bytes, 16-byte aligned (two calls that may run
- * at the same time need their own): with few rows the keys are split over CTAs and joined. */
+ * at the same time need their own): with few rows the keys are split over CTAs and joined.  How far goes by
+ * what the table can hold; a table as wide as its longest sequence is the fastest for short prompts.
+ * Values that are not finite cost time: rows that see none in a dim, next to one, are computed alone. */
 size_t qmtp_paged_prompt_workspace(const qmtp_paged_args* args, const qmtp_paged_cache* cache);
 int qmtp_paged_prompt(const qmtp_paged_args* args, const int* cu, const qmtp_paged_cache* cache, void* workspace,
                       size_t ws_bytes, void* stream);

@@ -553,8 +553,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constan
           for (int g = 0; g < KG; ++g) {
             const float p0 = ex2(__fmaf_rn(s[g][t][i], a.scale2, neg)), p1 = ex2(__fmaf_rn(s[g][t][i + 2], a.scale2, neg));
             sum = __fadd_rn(sum, __fadd_rn(p0, p1));
-            // the weights enter the second product as bf16 (relative error 2^-9 each, against the
-            // output's own bf16 rounding of the same size); their sum l keeps all 32 bits
+            // the weights enter the second product as bf16 (off by at most 2^-8 relative each, as the output's own
+            // rounding is); their sum l keeps all 32 bits
             sm.p[n][16 * KG * warp + 16 * g + oct] = __float2bfloat16_rn(p0);
             sm.p[n][16 * KG * warp + 16 * g + oct + 8] = __float2bfloat16_rn(p1);
           }

@@ -98,11 +98,12 @@ def append_qkv(qkv, cache: PagedCache, table, lens, cu=None, *, n_heads: int, ga
     qkv bf16 [T, >= width]: per row n_heads query heads (``gated``: (q, gate) pairs), then the key heads,
     then the value heads.  cu int32 [B + 1]: rows cu[b] .. cu[b+1] are sequence b's new tokens, the last
     ones of its lens[b]; None: the same number of rows for every sequence.  q_norm, k_norm bf16 [head_dim]
-    or None; cos, sin fp32 [positions, rotary / 2] or None (``qmtp.model.rope_tables``); the rotation turns
+    or None, each by itself; cos, sin fp32 [positions, rotary / 2] or None (``qmtp.model.rope_tables``); the rotation turns
     the first 2 * cos.shape[1] dims.  Everything is computed in fp32 and rounded once.
 
     -> (q bf16 [T, n_heads, head_dim], gate: a view [T, n_heads, head_dim] of qkv, or None).  Rows of no
-    sequence, and rows at a negative position (lens[b] below the row count), are left as they were."""
+    sequence, and rows at a negative position (lens[b] below the row count), are left as they were.  Offsets
+    that decrease or leave [0, T] hold no rows and set the device error word."""
     dev, dh = cache._index, cache.head_dim
     _tensor("qkv", qkv, BF16, dev)
     if qkv.dim() != 2:
@@ -215,7 +216,9 @@ def attention(q, cache: PagedCache, table, lens, *, gate=None, scale: float | No
     A query sees the keys at or before its position, with a window only those less than ``window`` back and
     the first ``sinks``; a query that sees none gives zeros.  scale: head_dim ** -0.5 by default.  gate (q's
     shape, any head and row strides): the result is multiplied by sigmoid(gate).  A token's result has the
-    same bits whatever the batch, S and the page size are.  out must not overlap the inputs."""
+    same bits whatever the batch, S and the page size are, as long as its sequence's keys and values are
+    finite.  out must not overlap the inputs.  The workspace goes by the table's width, not by the lengths:
+    a table much wider than its sequences costs memory, and a second launch where a short one needs one."""
     a, out = _attention_args(q, cache, gate, scale, window, sinks, out)
     if q.shape[0]:
         L = _lib.lib()
@@ -228,7 +231,8 @@ def prompt_attention(q, cache: PagedCache, table, lens, cu, *, gate=None, scale:
                      sinks: int = 0, out=None):
     """Attention of a ragged batch of prompt chunks: rows cu[b] .. cu[b+1] of q bf16 [T, heads, head_dim] are the
     last tokens of sequence b -> bf16 [T, heads * head_dim].  Masks, scale and gate as in ``attention``; rows of
-    no sequence are left as they were.  Any number of new tokens per sequence; ``attention`` is the one for a few."""
+    no sequence are left as they were.  Any number of new tokens per sequence; ``attention`` is the one for a few.
+    Short prompts are fastest with a table as wide as the longest sequence (the keys are split by its width)."""
     a, out = _attention_args(q, cache, gate, scale, window, sinks, out)
     if cu is None:
         _need(False, "a prompt's rows are named by cu")
