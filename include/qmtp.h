@@ -440,7 +440,8 @@ int qmtp_moe_dispatch(const void* idx, int T, int S, const void* x, int H, int n
  * lens[b] == 0 is empty.  Bad device-side values never read or write outside the arrays: they set bit 1
  * of the device error word, and a sequence whose length is negative or above table_w * page counts as
  * empty, a row of a page outside [0, pages) is read as zeros and not written, and a sequence whose row
- * offsets decrease or leave [0, T] has no rows (rows that two others then hold are either's). */
+ * offsets decrease or leave [0, T] has no rows (rows that two others then hold are either's, and the
+ * prompt form may leave rows as they were). */
 typedef struct qmtp_paged_cache {
   void* k;
   void* v;
